@@ -1,6 +1,6 @@
 """In-tree build of the native parts.
 
-* ``lib/libpla_b200.so``  — the CUDA kernels behind the C ABI of ``include/pla_b200.h``
+* ``lib/libpla_b200.so``  — the CUDA kernels behind the C ABI of ``include/*.h``
   (nvcc, sm_100a only, no torch).
 * ``lib/pla_b200_ops.so`` — the C++ host layer registered as PyTorch custom ops
   (``TORCH_LIBRARY(pla_b200, ...)``); it validates tensors, fills the POD
@@ -44,7 +44,7 @@ def _newer(target: Path, deps) -> bool:
 
 
 def _headers():
-    return list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [ROOT / "include" / "pla_b200.h"]
+    return list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + sorted((ROOT / "include").glob("*.h"))
 
 
 def build_native(force: bool = False, verbose: bool = False) -> Path:

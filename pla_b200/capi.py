@@ -1,7 +1,8 @@
-"""ctypes view of the C ABI in ``include/pla_b200.h`` (torch-free: plain pointers and sizes).
+"""ctypes view of the C ABI in ``include/pla_b200.h`` and ``include/pla_b200_attention.h`` (torch-free: plain pointers
+and sizes).
 
-Every argument structure of the header is mirrored here as a ``ctypes.Structure`` of the same name, built by
-reading the header itself, so the two cannot drift apart; ``check_layout`` compares every structure's size and
+Every argument structure of the headers is mirrored here as a ``ctypes.Structure`` of the same name, built by
+reading the headers themselves, so the two cannot drift apart; ``check_layout`` compares every structure's size and
 every field's offset with what the compiled library reports (``pla_b200_struct_size`` /
 ``pla_b200_field_offset``). A binding in another language would declare the same structures by hand.
 """
@@ -14,15 +15,17 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "lib" / "libpla_b200.so"
 HEADER_PATH = PKG.parent / "include" / "pla_b200.h"
+ATTENTION_HEADER_PATH = PKG.parent / "include" / "pla_b200_attention.h"
 
 _SCALARS = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "float": ctypes.c_float, "uint8_t": ctypes.c_uint8}
 
 
-def _parse_header(text: str):
+def _parse_header(text: str, known=()):
     """``typedef struct NAME { ... } NAME;`` blocks -> {name: [(field, ctype), ...]} in declaration order.
-    Field types the header uses: pointers (any), int32_t, int64_t, float, and earlier structures by value."""
+    Field types the headers use: pointers (any), int32_t, int64_t, float, and earlier structures by value (``known``: those
+    of a header that this one includes)."""
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    structs = {}
+    structs = dict(known)
     for name, body in re.findall(r"typedef\s+struct\s+(\w+)\s*\{(.*?)\}\s*\1\s*;", text, flags=re.S):
         fields = []
         for decl in body.split(";"):
@@ -50,13 +53,15 @@ def _parse_header(text: str):
                 else:
                     raise ValueError(f"{name}.{ident}: unknown field type {kind!r}")
                 fields.append((ident, ctype))
-        cls = type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": f"``{name}`` of include/pla_b200.h."})
+        cls = type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": f"``{name}`` of the C ABI."})
         structs[name] = {"class": cls, "fields": fields}
-    return structs
+    return {name: entry for name, entry in structs.items() if name not in known}
 
 
 STRUCTS = _parse_header(HEADER_PATH.read_text())
-globals().update({name: entry["class"] for name, entry in STRUCTS.items()})
+ATTENTION_STRUCTS = _parse_header(ATTENTION_HEADER_PATH.read_text(), STRUCTS)
+ALL_STRUCTS = {**STRUCTS, **ATTENTION_STRUCTS}
+globals().update({name: entry["class"] for name, entry in ALL_STRUCTS.items()})
 
 # short names used by the tests
 Index = STRUCTS["pla_b200_index"]["class"]
@@ -71,7 +76,8 @@ _ENTRY_ARGS = {
     "pla_b200_kda_fold_layers": "pla_b200_kda_fold_args", "pla_b200_kda_conv_scatter": "pla_b200_kda_conv_scatter_args",
     "pla_b200_kda_replay_plan": "pla_b200_kda_commit_args", "pla_b200_kda_replay_commit": "pla_b200_kda_commit_args",
     "pla_b200_kda_replay_plan_static": "pla_b200_kda_commit_args", "pla_b200_kda_decode_mega": "pla_b200_kda_mega_args",
-    "pla_b200_causal_conv_prefill": "pla_b200_conv_prefill_args",
+    "pla_b200_causal_conv_prefill": "pla_b200_conv_prefill_args", "pla_b200_block_tables": "pla_b200_block_tables_args",
+    "pla_b200_rotary": "pla_b200_rotary_args", "pla_b200_paged_decode": "pla_b200_paged_decode_args",
 }
 
 
@@ -83,7 +89,7 @@ def load() -> ctypes.CDLL:
     for name, struct in _ENTRY_ARGS.items():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
-        fn.argtypes = [ctypes.POINTER(STRUCTS[struct]["class"]), ctypes.c_void_p]
+        fn.argtypes = [ctypes.POINTER(ALL_STRUCTS[struct]["class"]), ctypes.c_void_p]
     lib.pla_b200_struct_size.restype = ctypes.c_int64
     lib.pla_b200_struct_size.argtypes = [ctypes.c_char_p]
     lib.pla_b200_field_offset.restype = ctypes.c_int64
@@ -92,6 +98,8 @@ def load() -> ctypes.CDLL:
     lib.pla_b200_gdn_chunk_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
     lib.pla_b200_kda_chunk_workspace_bytes.restype = ctypes.c_int64
     lib.pla_b200_kda_chunk_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32]
+    lib.pla_b200_paged_decode_workspace_bytes.restype = ctypes.c_int64
+    lib.pla_b200_paged_decode_workspace_bytes.argtypes = [ctypes.c_int32] * 4
     lib.pla_b200_device_status.restype = ctypes.c_int
     lib.pla_b200_device_status.argtypes = [ctypes.POINTER(ctypes.c_int32), ctypes.c_int]
     return lib
@@ -99,7 +107,7 @@ def load() -> ctypes.CDLL:
 
 def check_layout(lib: ctypes.CDLL) -> None:
     """Raises AssertionError when a mirrored structure differs from the compiled one in size or in any field offset."""
-    for name, entry in STRUCTS.items():
+    for name, entry in ALL_STRUCTS.items():
         cls = entry["class"]
         want = lib.pla_b200_struct_size(name.encode())
         assert want > 0, f"the library does not know {name}"
@@ -120,20 +128,20 @@ def index_of(tensor) -> "Index":
 
 def emit_layout() -> str:
     """Source of ``csrc/abi_layout.cu``: the table behind ``pla_b200_struct_size`` / ``pla_b200_field_offset``, one
-    ``offsetof`` per field of the header. Regenerate after changing the header:
+    ``offsetof`` per field of the headers. Regenerate after changing one:
     ``python -m pla_b200.capi --emit-layout``."""
     out = [
-        "// Sizes and field offsets of every argument structure of include/pla_b200.h, so that a binding which mirrors",
+        "// Sizes and field offsets of every argument structure of the include/ headers, so that a binding which mirrors",
         "// the structures in another language can check itself against the compiled library (the Python mirror does).",
-        "// Generated from the header, one line per field:  python -m pla_b200.capi --emit-layout",
-        "#include <stddef.h>", "#include <string.h>", "", '#include "../../include/pla_b200.h"', "", "namespace {",
+        "// Generated from the headers, one line per field:  python -m pla_b200.capi --emit-layout",
+        "#include <stddef.h>", "#include <string.h>", "", '#include "../../include/pla_b200_attention.h"', "", "namespace {",
         "struct FieldRow {", "  const char* type;", "  const char* field;", "  int64_t offset;", "};",
         "struct SizeRow {", "  const char* type;", "  int64_t size;", "};",
         "#define ROW(T, F) {#T, #F, static_cast<int64_t>(offsetof(T, F))}", "const FieldRow kFields[] = {"]
-    for name, entry in STRUCTS.items():
+    for name, entry in ALL_STRUCTS.items():
         out += [f"    ROW({name}, {field})," for field, _ in entry["fields"]]
     out += ["};", "const SizeRow kSizes[] = {"]
-    out += [f'    {{"{name}", static_cast<int64_t>(sizeof({name}))}},' for name in STRUCTS]
+    out += [f'    {{"{name}", static_cast<int64_t>(sizeof({name}))}},' for name in ALL_STRUCTS]
     out += ["};", "}  // namespace", "",
             'extern "C" int64_t pla_b200_struct_size(const char* type) {', "  if (type == nullptr) return -1;",
             "  for (const SizeRow& r : kSizes)", "    if (strcmp(r.type, type) == 0) return r.size;", "  return -1;", "}", "",
