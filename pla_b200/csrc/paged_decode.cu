@@ -1,97 +1,585 @@
 // Attention of one new token per request over a paged key/value cache.
 //
-// One pass over the keys with the running maximum and sum of the softmax: s = scale q.k (kept in units of log2 so that the
-// exponential is one instruction), on a new maximum the sum and the output so far are scaled down. One CTA per (request,
-// query head); its warps take the tokens in turn, a lane holds every 32nd channel, and the warps' maxima, sums and outputs are joined
-// at the end. Scores, sums and outputs are 32-bit; one rounding of the output.
+// One pass over the keys with the running maximum and sum of the softmax: s = scale q.k in units of log2 (the exponential is one
+// instruction), on a new maximum the sum and the output so far are scaled down. The call is bound by the bytes of the cache; with
+// eight query heads per key/value head, plain multiply-adds could not keep up with them (16 flops per byte and the conversions), so
+// both products run on the matrix unit: S^T = K Q^T with keys as rows, so that groups of up to eight heads waste nothing of an
+// m16n8k16 instruction, and O^T = V^T P^T. tcgen05 would want 128 keys by 8 heads in tensor memory and the softmax across its lanes; at
+// 24 bytes per cycle and SM the warp-level instruction is busy for a few percent of the time and keeps everything in registers.
+//
+// Work: units of 64 tokens of one (request, key/value head). Every CTA adds up the lengths itself and takes an equal, consecutive
+// range of all units (the lengths are on the device, so the host could not split them), which keeps the SMs equally loaded whatever
+// the lengths are and splits a single long request over all of them. In a unit each of the four warps takes 16 tokens, keeps its own
+// maxima, sums and output, and streams its rows through its own ring of shared memory: one bulk copy per row and lane (lanes 0-15
+// keys, 16-31 values), no barrier between warps until the range leaves the (request, head). Rows are 16 bytes longer in shared
+// memory than in the cache: ldmatrix reads eight rows without bank conflicts.
+// A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
+// waits on the first one's end only, joins the parts in order: no atomics, the same bits every time.
+// Scores, sums and outputs are 32-bit; the weights p are rounded to the activations' type for the product with V (relative 2^-8
+// or 2^-11, the same size as the output's own rounding), the sum of the weights is of the unrounded ones.
 #include "common.cuh"
 #include "../../include/pla_b200_attention.h"
 
 namespace pla {
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+constexpr int TILE = 16;              // tokens per warp and step
+constexpr int UNIT = TILE * WARPS;    // tokens per CTA and step
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr float SLACK = 8.0f;         // the running maximum may lag this far (log2) behind: p stays below 2^8, fewer rescalings
 
-template <typename act_t, int D>
-__global__ void __launch_bounds__(WARPS * 32) paged_decode_kernel(const pla_b200_paged_decode_args p) {
-  constexpr int E = D / 32;
-  __shared__ float s_m[WARPS], s_l[WARPS], s_o[WARPS][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t b = blockIdx.x / p.Hq;
-  const int h = blockIdx.x % p.Hq, hk = h / (p.Hq / p.Hk);
-  const act_t* q = static_cast<const act_t*>(p.q) + b * p.q_row_stride + h * p.q_head_stride;
-  const act_t* kc = static_cast<const act_t*>(p.k_cache) + hk * p.k_strides.head;
-  const act_t* vc = static_cast<const act_t*>(p.v_cache) + hk * p.v_strides.head;
-  int64_t len = p.seq_lens[b];
-  int32_t bad = 0;
-  if (len < 0) bad |= PLA_B200_DEV_BAD_INTERVAL, len = 0;
-  const int64_t room = static_cast<int64_t>(p.columns) * p.block_size;
-  if (len > room) bad |= PLA_B200_DEV_BAD_INTERVAL, len = room;
-  float qs[E], o[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    qs[i] = to_f32(q[lane + 32 * i]) * p.scale * LOG2E;
-    o[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = warp; j < len; j += WARPS) {
-    const int64_t page = p.block_table[b * p.table_row_stride + j / p.block_size];
-    if (page < 0 || page >= p.num_blocks) {
-      bad |= PLA_B200_DEV_BAD_SLOT;
-      continue;
-    }
-    const int64_t in = j % p.block_size;
-    const act_t* k = kc + page * p.k_strides.block + in * p.k_strides.token;
-    const act_t* v = vc + page * p.v_strides.block + in * p.v_strides.token;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) s += qs[i] * to_f32(k[lane + 32 * i]);
-    s = warp_sum(s);
-    const float top = fmaxf(m, s);
-    const float down = top == -INFINITY ? 1.0f : exp2f(m - top), w = top == -INFINITY ? 0.0f : exp2f(s - top);
-    m = top;
-    l = l * down + w;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = o[i] * down + w * to_f32(v[lane + 32 * i]);
-  }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-  for (int i = 0; i < E; ++i) s_o[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < WARPS; ++w) sum += s_m[w] == -INFINITY ? 0.0f : s_l[w] * exp2f(s_m[w] - top);
-  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
-    float x = 0.0f;
-    for (int w = 0; w < WARPS; ++w) x += s_m[w] == -INFINITY ? 0.0f : s_o[w][d] * exp2f(s_m[w] - top);
-    static_cast<act_t*>(p.out)[(b * p.Hq + h) * D + d] = from_f32<act_t>(sum == 0.0f ? 0.0f : x / sum);
-  }
-  if (threadIdx.x == 0 && p.lse != nullptr) p.lse[b * p.Hq + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
-  if (bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
+// Shared memory per CTA that leaves as many CTAs on an SM as the ring's depth allows: three stages each.
+constexpr int STAGES = 3;
+template <int D>
+struct Shape {
+  static constexpr int PITCH = D * 2 + 16;                 // bytes per row
+  static constexpr int ROWS = TILE * PITCH;                // keys (or values) of a tile
+  static constexpr int STAGE = 2 * ROWS;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int HALF = D / 2;
+  static constexpr int OP = HALF + 4;                      // row pitch (floats) of the join buffer
+  static constexpr int JOIN = WARPS * 8 * OP * 4;
+  static constexpr int SMEM = RING + JOIN;
+  static constexpr int CTAS = SMEM > 113 * 1024 ? 1 : SMEM > 75 * 1024 ? 2 : SMEM > 56 * 1024 ? 3 : 4;   // of 227 KB
+};
+
+struct Plan {              // of one call, the same on host and device
+  int chunks;              // groups of 8 * NT query heads per key/value head
+  int group;               // query heads per key/value head
+  int grid;
+  float* part_o;           // [2 * grid][8 * NT][D]
+  float* part_m;           // [2 * grid][8 * NT]
+  float* part_l;
+  int4* head_part;         // [grid]: {request, head item, last CTA that holds a part of it, 1}; w = 0: nothing begins here and goes on
+};
+
+template <typename act_t>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 template <typename act_t>
-void launch(const pla_b200_paged_decode_args& a, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hq);
-  switch (a.D) {
-    case 64: paged_decode_kernel<act_t, 64><<<grid, WARPS * 32, 0, s>>>(a); break;
-    case 96: paged_decode_kernel<act_t, 96><<<grid, WARPS * 32, 0, s>>>(a); break;
-    case 128: paged_decode_kernel<act_t, 128><<<grid, WARPS * 32, 0, s>>>(a); break;
-    case 192: paged_decode_kernel<act_t, 192><<<grid, WARPS * 32, 0, s>>>(a); break;
-    default: paged_decode_kernel<act_t, 256><<<grid, WARPS * 32, 0, s>>>(a); break;
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float* c, const uint32_t* a, const uint32_t* b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float* c, const uint32_t* a, const uint32_t* b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ int length_of(const pla_b200_paged_decode_args& p, int b, int32_t& bad) {
+  const int64_t room = min(static_cast<int64_t>(p.columns) * p.block_size, static_cast<int64_t>(1) << 30);
+  const int n = p.seq_lens[b];
+  if (n < 0 || n > room) bad |= PLA_B200_DEV_BAD_INTERVAL;
+  return n < 0 ? 0 : n > room ? static_cast<int>(room) : n;
+}
+
+// A place in the sequence of units: request, (key/value head, chunk) item of it, unit of the item.
+struct Place {
+  int b, item, unit, units, len;
+};
+
+__device__ __forceinline__ void advance(Place& x, const pla_b200_paged_decode_args& p, int items) {
+  if (++x.unit < x.units) return;
+  x.unit = 0;
+  if (++x.item < items) return;
+  x.item = 0;
+  int32_t ignored = 0;
+  do {
+    if (++x.b >= p.B) {                 // past the end: the caller counts its units and never uses this place
+      x.units = 1 << 30;
+      x.len = 0;
+      return;
+    }
+    x.len = length_of(p, x.b, ignored);
+    x.units = (x.len + UNIT - 1) / UNIT;
+  } while (x.units == 0);
+}
+
+template <typename act_t, int D, int NT>
+__global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan) {
+  using S = Shape<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t s_full[WARPS][STAGES];
+  __shared__ uint32_t s_live[WARPS][STAGES];
+  __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
+  __shared__ int64_t s_scan[WARPS];
+  __shared__ int64_t s_total;
+  __shared__ int s_place[3];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int items = p.Hk * plan.chunks;
+  int32_t bad = 0;
+
+  // ---- the CTA's range of units
+  const int per = (p.B + THREADS - 1) / THREADS;
+  const int lo = min(tid * per, p.B), hi = min(lo + per, p.B);
+  int64_t mine = 0;
+  for (int b = lo; b < hi; ++b) mine += (length_of(p, b, bad) + UNIT - 1) / UNIT;
+  mine *= items;
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&s_full[warp][i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) upto += s_scan[w];
+    total += s_scan[w];
+  }
+  // requests of length zero are nobody's unit
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    int32_t ignored = 0;
+    if (length_of(p, b, ignored) != 0) continue;
+    act_t* o = static_cast<act_t*>(p.out) + static_cast<int64_t>(b) * p.Hq * D;
+    for (int i = tid; i < p.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
+    if (p.lse != nullptr)
+      for (int i = tid; i < p.Hq; i += THREADS) p.lse[static_cast<int64_t>(b) * p.Hq + i] = -INFINITY;
+  }
+  const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
+  if (blockIdx.x >= workers) {
+    if (tid == 0) plan.head_part[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (blockIdx.x == 0 && bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
+    return;
+  }
+  const int64_t begin = blockIdx.x * total / workers, end = (blockIdx.x + 1) * total / workers;
+  if (begin >= upto - mine && begin < upto) {
+    int64_t left = begin - (upto - mine);
+    for (int b = lo; b < hi; ++b) {
+      int32_t ignored = 0;
+      const int64_t units = (length_of(p, b, ignored) + UNIT - 1) / UNIT;
+      if (left < units * items) {
+        s_place[0] = b;
+        s_place[1] = static_cast<int>(left / units);
+        s_place[2] = static_cast<int>(left % units);
+        break;
+      }
+      left -= units * items;
+    }
+  }
+  __syncthreads();
+  Place at;
+  at.b = s_place[0];
+  at.item = s_place[1];
+  at.unit = s_place[2];
+  {
+    int32_t ignored = 0;
+    at.len = length_of(p, at.b, ignored);
+    at.units = (at.len + UNIT - 1) / UNIT;
+  }
+  const int count = static_cast<int>(end - begin);
+
+  // ---- loads: lane r < 16 brings key row r of the warp's tile, lane 16 + r value row r
+  uint8_t* ring = smem + warp * (STAGES * S::STAGE);
+  const int row = lane & 15;
+  const bool is_v = lane >= 16;
+  const pla_b200_page_strides st = is_v ? p.v_strides : p.k_strides;
+  const act_t* const cache = static_cast<const act_t*>(is_v ? p.v_cache : p.k_cache);
+  Place ahead = at;
+  int issued = 0;
+  auto page_of = [&](const Place& x) -> int {     // page of the lane's row, -1 past the end
+    const int t = x.unit * UNIT + warp * TILE + row;
+    return t < x.len ? p.block_table[x.b * p.table_row_stride + t / p.block_size] : -1;
+  };
+  int page = page_of(ahead);
+  auto issue = [&](int stage) {
+    const int t = ahead.unit * UNIT + warp * TILE + row;
+    const bool inside = t < ahead.len;
+    const bool live = inside && page >= 0 && page < p.num_blocks;
+    if (inside && !live) bad |= PLA_B200_DEV_BAD_SLOT;
+    const act_t* src = cache + page * st.block + (t % p.block_size) * st.token + (ahead.item / plan.chunks) * st.head;
+    uint8_t* dst = ring + stage * S::STAGE + lane * S::PITCH;
+    const uint32_t rows = __ballot_sync(0xffffffffu, live);
+    ++issued;
+    if (issued < count) {
+      advance(ahead, p, items);
+      page = page_of(ahead);                      // used one step later
+    }
+    if (!live && is_v) {                          // p = 0 there, but 0 * garbage need not be 0
+      for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+    }
+    fence_async_smem();
+    if (lane == 0) {
+      s_live[warp][stage] = rows;
+      mbar_expect_tx(&s_full[warp][stage], __popc(rows) * (D * 2));
+    }
+    __syncwarp();
+    if (live) bulk_load(dst, src, D * 2, &s_full[warp][stage]);
+  };
+  for (int i = 0; i < min(STAGES, count); ++i) issue(i);
+
+  // ---- the lane's part of the running state: heads 2 (lane % 4) and the next of each group of eight
+  float m[NT][2], l[NT][2], o[D / 16][NT][4];
+  uint32_t qf[D / 16][NT][2];
+  const float to_log2 = p.scale * LOG2E;
+  auto load_q = [&](const Place& x) {
+    const int chunk = x.item % plan.chunks, head = (x.item / plan.chunks) * plan.group + chunk * 8 * NT;
+    const int heads = min(8 * NT, plan.group - chunk * 8 * NT);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = n * 8 + lane / 4;
+      const act_t* q = static_cast<const act_t*>(p.q) + x.b * p.q_row_stride + (head + h) * p.q_head_stride + (lane % 4) * 2;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][n][0] = h < heads ? *reinterpret_cast<const uint32_t*>(q + kk * 16) : 0;
+        qf[kk][n][1] = h < heads ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) : 0;
+      }
+    }
+  };
+  auto clear = [&] {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[kk][n][i] = 0.0f;
+    }
+  };
+
+  // Joins the four warps' parts of the item that ends here (or leaves the range) and stores them.
+  auto flush = [&](const Place& x, bool whole, int slot) {
+    const int chunk = x.item % plan.chunks, head = (x.item / plan.chunks) * plan.group + chunk * 8 * NT;
+    const int heads = min(8 * NT, plan.group - chunk * 8 * NT);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], s);
+        if (lane < 4) {
+          s_m[warp][n * 8 + lane * 2 + i] = m[n][i];
+          s_l[warp][n * 8 + lane * 2 + i] = l[n][i];
+        }
+      }
+    __syncthreads();
+    float* join = reinterpret_cast<float*>(smem + S::RING);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float down[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY;
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][n * 8 + (lane % 4) * 2 + i]);
+        down[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - top);
+      }
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        float* mine = join + warp * 8 * S::OP;
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+          const float* c = o[part * (D / 32) + kk][n];
+          float* to = mine + (lane % 4) * 2 * S::OP + kk * 16 + lane / 4;
+          to[0] = c[0] * down[0];
+          to[S::OP] = c[1] * down[1];
+          to[8] = c[2] * down[0];
+          to[S::OP + 8] = c[3] * down[1];
+        }
+        __syncthreads();
+        for (int i = tid; i < 8 * S::HALF; i += THREADS) {
+          const int h = i / S::HALF, d = i % S::HALF, hh = n * 8 + h;
+          if (hh >= heads) continue;
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) sum += join[(w * 8 + h) * S::OP + d];
+          float top = -INFINITY, weight = 0.0f;
+          for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][hh]);
+          for (int w = 0; w < WARPS; ++w) weight += s_m[w][hh] == -INFINITY ? 0.0f : s_l[w][hh] * fast_exp2(s_m[w][hh] - top);
+          const bool first = part == 0 && d == 0;
+          if (whole) {
+            const int64_t out = static_cast<int64_t>(x.b) * p.Hq + head + hh;
+            static_cast<act_t*>(p.out)[out * D + part * S::HALF + d] = from_f32<act_t>(weight == 0.0f ? 0.0f : sum / weight);
+            if (first && p.lse != nullptr) p.lse[out] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
+          } else {
+            const int64_t to = static_cast<int64_t>(slot) * 8 * NT + hh;
+            plan.part_o[to * D + part * S::HALF + d] = sum;
+            if (first) plan.part_m[to] = top, plan.part_l[to] = weight;
+          }
+        }
+        __syncthreads();
+      }
+    }
+  };
+
+  int4 begins = make_int4(0, 0, 0, 0);
+  int first_unit = at.unit;
+  clear();
+  load_q(at);
+  bool timed_out = false;
+  for (int i = 0; i < count; ++i) {
+    const int stage = i % STAGES;
+    if (!timed_out) timed_out = __any_sync(0xffffffffu, !mbar_wait(&s_full[warp][stage], (i / STAGES) & 1));
+    const uint32_t live = s_live[warp][stage];
+    const uint32_t k_rows = smem_addr(ring + stage * S::STAGE), v_rows = k_rows + S::ROWS;
+    if (live != 0 && !timed_out) {
+      // scores of 16 tokens: lane holds tokens lane / 4 and + 8, heads 2 (lane % 4) and + 1
+      float s[NT][2][4] = {};
+      const uint32_t ka = k_rows + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        ldmatrix4(a, ka + kk * 32);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma<act_t>(s[n][kk & 1], a, qf[kk][n]);
+      }
+      const bool on0 = (live >> (lane / 4)) & 1, on1 = (live >> (lane / 4 + 8)) & 1;
+      uint32_t pf[NT][2];
+      float next[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* c = s[n][0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = (e < 2 ? on0 : on1) ? (c[e] + s[n][1][e]) * to_log2 : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(c[e], c[e + 2]);
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+          next[n][e] = x;
+          grow |= x > m[n][e] + SLACK;
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float down[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float top = fmaxf(m[n][e], next[n][e]);
+            down[e] = m[n][e] == -INFINITY ? 0.0f : fast_exp2(m[n][e] - top);
+            m[n][e] = top;
+            l[n][e] *= down[e];
+          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            o[kk][n][0] *= down[0];
+            o[kk][n][1] *= down[1];
+            o[kk][n][2] *= down[0];
+            o[kk][n][3] *= down[1];
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* c = s[n][0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float top = m[n][e & 1];
+          c[e] = fast_exp2(c[e] - (top == -INFINITY ? 0.0f : top));
+          l[n][e & 1] += c[e];
+        }
+        pf[n][0] = transpose8x8(pack2<act_t>(c[0], c[1]));
+        pf[n][1] = transpose8x8(pack2<act_t>(c[2], c[3]));
+      }
+      const uint32_t va = v_rows + ((lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        ldmatrix4_trans(a, va + kk * 32);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma<act_t>(o[kk][n], a, pf[n]);
+      }
+    }
+    __syncwarp();
+    if (issued < count && !timed_out) issue(stage);
+    if (at.unit + 1 == at.units || i + 1 == count) {
+      const bool whole = first_unit == 0 && at.unit + 1 == at.units;
+      if (first_unit == 0 && !whole) {
+        // this part begins the item: name the last CTA that goes on with it
+        const int64_t item_end = end + (at.units - 1 - at.unit);
+        begins = make_int4(at.b, at.item, static_cast<int>((item_end * workers - 1) / total), 1);
+      }
+      flush(at, whole, 2 * blockIdx.x + (first_unit == 0 ? 1 : 0));
+      clear();
+      first_unit = 0;
+      const int item = at.item, b = at.b;
+      advance(at, p, items);
+      if (i + 1 < count && (item != at.item || b != at.b)) load_q(at);
+    } else {
+      ++at.unit;
+    }
+  }
+  if (timed_out) {                       // a copy never came: say so, and give the others time to land before the CTA's memory goes
+    bad |= PLA_B200_DEV_WAIT_TIMEOUT;
+    for (int i = max(issued - STAGES, 0); i < issued; ++i) mbar_wait(&s_full[warp][i % STAGES], (i / STAGES) & 1);
+  }
+  if (tid == 0) plan.head_part[blockIdx.x] = begins;
+  if (bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
+}
+
+// Joins the parts of every item that lies in several CTAs' ranges: CTA (i, h) that of the item which begins in the range of CTA i, head h.
+template <typename act_t, int D, int NT>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(const pla_b200_paged_decode_args p, const Plan plan) {
+  constexpr int VEC = D / 4, GROUPS = THREADS / VEC;     // threads per part, parts read at a time
+  __shared__ float s_red[WARPS];
+  __shared__ float4 s_o[GROUPS][VEC];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 begins = plan.head_part[blockIdx.x];
+  if (begins.w == 0) return;
+  const int chunk = begins.y % plan.chunks, h = blockIdx.y;
+  if (h >= min(8 * NT, plan.group - chunk * 8 * NT)) return;
+  const int i = blockIdx.x, parts = begins.z - i + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto index = [&](int j) -> int64_t { return static_cast<int64_t>(j == 0 ? 2 * i + 1 : 2 * (i + j)) * 8 * NT + h; };
+  float top = -INFINITY;
+  for (int j = tid; j < parts; j += THREADS) top = fmaxf(top, plan.part_m[index(j)]);
+#pragma unroll
+  for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+  if (lane == 0) s_red[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_red[w]);
+  __syncthreads();
+  float weight = 0.0f;
+  for (int j = tid; j < parts; j += THREADS) {
+    const float m = plan.part_m[index(j)];
+    if (m != -INFINITY) weight += plan.part_l[index(j)] * fast_exp2(m - top);
+  }
+  weight = warp_sum(weight);
+  if (lane == 0) s_red[warp] = weight;
+  const int g = tid / VEC, d = tid % VEC;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (g < GROUPS) {
+    for (int j = g; j < parts; j += GROUPS) {
+      const float m = plan.part_m[index(j)];
+      const float f = m == -INFINITY ? 0.0f : fast_exp2(m - top);
+      const float4 x = reinterpret_cast<const float4*>(plan.part_o + index(j) * D)[d];
+      sum.x += x.x * f, sum.y += x.y * f, sum.z += x.z * f, sum.w += x.w * f;
+    }
+    s_o[g][d] = sum;
+  }
+  __syncthreads();
+  weight = 0.0f;
+  for (int w = 0; w < WARPS; ++w) weight += s_red[w];
+  if (tid < VEC) {
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k) {
+      const float4 x = s_o[k][tid];
+      sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    const float f = weight == 0.0f ? 0.0f : 1.0f / weight;
+    const int64_t out = static_cast<int64_t>(begins.x) * p.Hq + (begins.y / plan.chunks) * plan.group + chunk * 8 * NT + h;
+    uint2 raw = make_uint2(pack2<act_t>(sum.x * f, sum.y * f), pack2<act_t>(sum.z * f, sum.w * f));
+    *reinterpret_cast<uint2*>(static_cast<act_t*>(p.out) + out * D + tid * 4) = raw;
+    if (tid == 0 && p.lse != nullptr) p.lse[out] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
   }
 }
 
+int tiles_of(int group) { return group <= 8 ? 1 : 2; }     // n-tiles of eight heads that a warp keeps at once
+
+template <int D>
+int full_grid() { return sm_count() * Shape<D>::CTAS; }
+
+int full_grid_of(int D) {
+  return D == 64 ? full_grid<64>() : D == 96 ? full_grid<96>() : D == 128 ? full_grid<128>() : D == 192 ? full_grid<192>() : full_grid<256>();
+}
+
+int64_t workspace_bytes(int grid, int NT, int D) {
+  return static_cast<int64_t>(grid) * sizeof(int4) + static_cast<int64_t>(2 * grid) * 8 * NT * (D + 2) * 4;
+}
+
+template <typename act_t, int D, int NT>
+int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
+  using S = Shape<D>;
+  static DeviceOnce once;
+  int dev = 0;
+  PLA_CUDA_OK(cudaGetDevice(&dev));
+  if (once.needed(dev)) {
+    PLA_CUDA_OK(cudaFuncSetAttribute(paged_decode_kernel<act_t, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    once.mark(dev);
+  }
+  Plan plan;
+  plan.group = a.Hq / a.Hk;
+  plan.chunks = (plan.group + 8 * NT - 1) / (8 * NT);
+  // No more units than this, and one per (request, item) when no table row holds more than 64 tokens.
+  const int64_t items = static_cast<int64_t>(a.B) * a.Hk * plan.chunks;
+  const int64_t per_item = (static_cast<int64_t>(a.columns) * a.block_size + UNIT - 1) / UNIT;
+  const int64_t units = per_item > (INT64_MAX / items) ? INT64_MAX : items * per_item;
+  plan.grid = static_cast<int>(units < 1 ? 1 : units < full_grid<D>() ? units : full_grid<D>());
+  plan.head_part = static_cast<int4*>(a.workspace);
+  plan.part_o = reinterpret_cast<float*>(plan.head_part + plan.grid);
+  plan.part_m = plan.part_o + static_cast<int64_t>(2 * plan.grid) * 8 * NT * D;
+  plan.part_l = plan.part_m + static_cast<int64_t>(2 * plan.grid) * 8 * NT;
+  PLA_REQUIRE(a.workspace_bytes >= workspace_bytes(plan.grid, NT, D), PLA_B200_E_INVALID, "the workspace is too small");
+  paged_decode_kernel<act_t, D, NT><<<plan.grid, THREADS, S::SMEM, stream>>>(a, plan);
+  PLA_CUDA_OK(cudaGetLastError());
+  if (per_item > 1) {                               // else every item is one unit and was stored whole
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.grid, plan.group < 8 * NT ? plan.group : 8 * NT);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PLA_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<act_t, D, NT>, a, plan));
+  }
+  return PLA_B200_OK;
+}
+
+template <typename act_t>
+int launch_for(const pla_b200_paged_decode_args& a, cudaStream_t s) {
+  const bool one = tiles_of(a.Hq / a.Hk) == 1;
+  switch (a.D) {
+    case 64: return one ? launch<act_t, 64, 1>(a, s) : launch<act_t, 64, 2>(a, s);
+    case 96: return one ? launch<act_t, 96, 1>(a, s) : launch<act_t, 96, 2>(a, s);
+    case 128: return one ? launch<act_t, 128, 1>(a, s) : launch<act_t, 128, 2>(a, s);
+    case 192: return one ? launch<act_t, 192, 1>(a, s) : launch<act_t, 192, 2>(a, s);
+    default: return one ? launch<act_t, 256, 1>(a, s) : launch<act_t, 256, 2>(a, s);
+  }
+}
+
+bool head_size_ok(int D) { return D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
 bool strides16(const pla_b200_page_strides& s) { return s.block % 8 == 0 && s.token % 8 == 0 && s.head % 8 == 0; }
 
 }  // namespace
 }  // namespace pla
 
 extern "C" int64_t pla_b200_paged_decode_workspace_bytes(int32_t B, int32_t Hq, int32_t Hk, int32_t D) {
-  if (B < 0 || Hq <= 0 || Hk <= 0 || D <= 0) return -1;
-  return 0;
+  using namespace pla;
+  if (B < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || !head_size_ok(D)) return -1;
+  return workspace_bytes(full_grid_of(D), tiles_of(Hq / Hk), D);
 }
 
 extern "C" int pla_b200_paged_decode(const pla_b200_paged_decode_args* args, void* stream) {
@@ -101,20 +589,16 @@ extern "C" int pla_b200_paged_decode(const pla_b200_paged_decode_args* args, voi
   default_status(a);
   PLA_REQUIRE(a.B >= 0 && a.Hq > 0 && a.Hk > 0 && a.Hq % a.Hk == 0, PLA_B200_E_INVALID,
               "paged decode needs B >= 0 and a positive number of query heads that the key/value heads divide");
-  PLA_REQUIRE(a.D == 64 || a.D == 96 || a.D == 128 || a.D == 192 || a.D == 256, PLA_B200_E_UNSUPPORTED,
-              "the head size must be 64, 96, 128, 192 or 256");
+  PLA_REQUIRE(head_size_ok(a.D), PLA_B200_E_UNSUPPORTED, "the head size must be 64, 96, 128, 192 or 256");
   PLA_REQUIRE(a.act_dtype == PLA_B200_BF16 || a.act_dtype == PLA_B200_F16, PLA_B200_E_INVALID, "paged decode takes bf16 or fp16");
   if (a.B == 0) return PLA_B200_OK;
   PLA_REQUIRE(static_cast<int64_t>(a.B) * a.Hq <= INT32_MAX, PLA_B200_E_TOO_LARGE, "too many rows");
   PLA_REQUIRE(a.columns >= 0 && a.block_size > 0 && a.num_blocks >= 0, PLA_B200_E_INVALID, "bad block table sizes");
-  PLA_REQUIRE(a.q && a.out && a.seq_lens && (a.columns == 0 || a.block_table) && (a.num_blocks == 0 || (a.k_cache && a.v_cache)),
-              PLA_B200_E_INVALID, "q, the caches, block_table, seq_lens and out are required");
-  PLA_REQUIRE(aligned16(a.q) && aligned16(a.k_cache) && aligned16(a.v_cache) && aligned16(a.out) && a.q_row_stride % 8 == 0 &&
+  PLA_REQUIRE(a.q && a.out && a.seq_lens && (a.columns == 0 || a.block_table) && (a.num_blocks == 0 || (a.k_cache && a.v_cache)) && a.workspace,
+              PLA_B200_E_INVALID, "q, the caches, block_table, seq_lens, out and the workspace are required");
+  PLA_REQUIRE(aligned16(a.q) && aligned16(a.k_cache) && aligned16(a.v_cache) && aligned16(a.out) && aligned16(a.workspace) && a.q_row_stride % 8 == 0 &&
                   a.q_head_stride % 8 == 0 && strides16(a.k_strides) && strides16(a.v_strides),
-              PLA_B200_E_ALIGN, "q, out and cache rows must be 16-byte aligned");
+              PLA_B200_E_ALIGN, "q, out, workspace and cache rows must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.act_dtype == PLA_B200_BF16) launch<__nv_bfloat16>(a, s);
-  else launch<__half>(a, s);
-  PLA_CUDA_OK(cudaGetLastError());
-  return PLA_B200_OK;
+  return a.act_dtype == PLA_B200_BF16 ? launch_for<__nv_bfloat16>(a, s) : launch_for<__half>(a, s);
 }
