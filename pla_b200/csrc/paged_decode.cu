@@ -10,13 +10,17 @@
 // Work: units of 64 tokens of one (request, key/value head). Every CTA adds up the lengths itself and takes an equal, consecutive
 // range of all units (the lengths are on the device, so the host could not split them), which keeps the SMs equally loaded whatever
 // the lengths are and splits a single long request over all of them. In a unit each of the four warps takes 16 tokens, keeps its own
-// maxima, sums and output, and streams its rows through its own ring of shared memory: one bulk copy per row and lane (lanes 0-15
-// keys, 16-31 values), no barrier between warps until the range leaves the (request, head). Rows are 16 bytes longer in shared
-// memory than in the cache: ldmatrix reads eight rows without bank conflicts.
+// maxima, sums and output, and streams its rows through its own ring of shared memory, without a barrier between warps until the
+// range leaves the (request, head). Where pages hold whole tiles of 16 tokens, a tile is a box of a tensor map over the cache and one
+// lane brings it with a copy per 64 channels; other page sizes take 16-byte asynchronous copies from each row's page. (One bulk copy
+// per row and lane was tried first: the 32 lanes' copies issue one after another, 480 of 620 instructions per tile; 256 us where
+// the boxes take XXX for 64 requests up to 16K tokens of D = 256.) Both leave the 128-byte swizzle that ldmatrix reads without bank conflicts.
 // A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
 // waits on the first one's end only, joins the parts in order: no atomics, the same bits every time.
 // Scores, sums and outputs are 32-bit; the weights p are rounded to the activations' type for the product with V (relative 2^-8
 // or 2^-11, the same size as the output's own rounding), the sum of the weights is of the unrounded ones.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "../../include/pla_b200_attention.h"
 
@@ -31,19 +35,20 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float SLACK = 8.0f;         // the running maximum may lag this far (log2) behind: p stays below 2^8, fewer rescalings
 
-// Shared memory per CTA that leaves as many CTAs on an SM as the ring's depth allows: three stages each.
-constexpr int STAGES = 3;
+// Ring depth per warp, and CTAs per SM that its shared memory leaves room for (of 227 KB): at least 96 KB in flight per SM.
 template <int D>
 struct Shape {
-  static constexpr int PITCH = D * 2 + 16;                 // bytes per row
-  static constexpr int ROWS = TILE * PITCH;                // keys (or values) of a tile
+  static constexpr int BOXES = (D + 63) / 64;              // 64 channels of 16 rows each: 2 KB
+  static constexpr int BOX = TILE * 128;
+  static constexpr int ROWS = BOXES * BOX;                 // keys (or values) of a tile
   static constexpr int STAGE = 2 * ROWS;
+  static constexpr int STAGES = D == 64 ? 4 : 3;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int HALF = D / 2;
   static constexpr int OP = HALF + 4;                      // row pitch (floats) of the join buffer
   static constexpr int JOIN = WARPS * 8 * OP * 4;
-  static constexpr int SMEM = RING + JOIN;
-  static constexpr int CTAS = SMEM > 113 * 1024 ? 1 : SMEM > 75 * 1024 ? 2 : SMEM > 56 * 1024 ? 3 : 4;   // of 227 KB
+  static constexpr int SMEM = 1024 + RING + JOIN;          // the ring begins at a multiple of 1,024 bytes
+  static constexpr int CTAS = SMEM > 113 * 1024 ? 1 : SMEM > 75 * 1024 ? 2 : 3;
 };
 
 struct Plan {              // of one call, the same on host and device
@@ -100,6 +105,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
+// Box of a cache tensor map: channels from x of one head, TILE tokens of one page, into swizzled shared memory.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, int page, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(token), "r"(page), "r"(smem_addr(bar))
+               : "memory");
+}
+// 16 bytes from global memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// Arrives on `bar` once the thread's earlier copy16()s have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
 __device__ __forceinline__ int length_of(const pla_b200_paged_decode_args& p, int b, int32_t& bad) {
   const int64_t room = min(static_cast<int64_t>(p.columns) * p.block_size, static_cast<int64_t>(1) << 30);
   const int n = p.seq_lens[b];
@@ -129,10 +149,15 @@ __device__ __forceinline__ void advance(Place& x, const pla_b200_paged_decode_ar
   } while (x.units == 0);
 }
 
-template <typename act_t, int D, int NT>
-__global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan) {
+// BOXED: pages hold whole tiles, the maps describe the caches.
+template <typename act_t, int D, int NT, bool BOXED>
+__global__ void __launch_bounds__(THREADS, Shape<D>::CTAS)
+paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const __grid_constant__ CUtensorMap k_map,
+                    const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D>;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   __shared__ uint64_t s_full[WARPS][STAGES];
   __shared__ uint32_t s_live[WARPS][STAGES];
   __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
@@ -158,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(c
   }
   if (lane == 31) s_scan[warp] = upto;
   if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&s_full[warp][i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&s_full[warp][i], BOXED ? 1 : 32);
     fence_mbar_init();
   }
   __syncthreads();
@@ -209,42 +234,57 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(c
   }
   const int count = static_cast<int>(end - begin);
 
-  // ---- loads: lane r < 16 brings key row r of the warp's tile, lane 16 + r value row r
+  // ---- loads
   uint8_t* ring = smem + warp * (STAGES * S::STAGE);
-  const int row = lane & 15;
-  const bool is_v = lane >= 16;
-  const pla_b200_page_strides st = is_v ? p.v_strides : p.k_strides;
-  const act_t* const cache = static_cast<const act_t*>(is_v ? p.v_cache : p.k_cache);
+  const uint32_t ring_addr = smem_addr(ring);
   Place ahead = at;
   int issued = 0;
-  auto page_of = [&](const Place& x) -> int {     // page of the lane's row, -1 past the end
+  // The lane's token of the tile: all lanes the first one's when it comes as a box, else lanes r and r + 16 row r's (keys and values).
+  const int row = BOXED ? 0 : lane & 15;
+  auto page_of = [&](const Place& x) -> int {     // -1 past the end
     const int t = x.unit * UNIT + warp * TILE + row;
     return t < x.len ? p.block_table[x.b * p.table_row_stride + t / p.block_size] : -1;
   };
   int page = page_of(ahead);
   auto issue = [&](int stage) {
-    const int t = ahead.unit * UNIT + warp * TILE + row;
-    const bool inside = t < ahead.len;
-    const bool live = inside && page >= 0 && page < p.num_blocks;
-    if (inside && !live) bad |= PLA_B200_DEV_BAD_SLOT;
-    const act_t* src = cache + page * st.block + (t % p.block_size) * st.token + (ahead.item / plan.chunks) * st.head;
-    uint8_t* dst = ring + stage * S::STAGE + lane * S::PITCH;
-    const uint32_t rows = __ballot_sync(0xffffffffu, live);
+    const int t = ahead.unit * UNIT + warp * TILE + row, in = t % p.block_size, head = ahead.item / plan.chunks, left = ahead.len - t;
+    const bool live = left > 0 && page >= 0 && page < p.num_blocks;
+    if (left > 0 && !live) bad |= PLA_B200_DEV_BAD_SLOT;
+    const uint32_t to = ring_addr + stage * S::STAGE;
+    uint64_t* const bar = &s_full[warp][stage];
+    const int from = page;
     ++issued;
     if (issued < count) {
       advance(ahead, p, items);
       page = page_of(ahead);                      // used one step later
     }
-    if (!live && is_v) {                          // p = 0 there, but 0 * garbage need not be 0
-      for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
-    }
-    fence_async_smem();
-    if (lane == 0) {
-      s_live[warp][stage] = rows;
-      mbar_expect_tx(&s_full[warp][stage], __popc(rows) * (D * 2));
+    if constexpr (BOXED) {
+      if (lane == 0) {
+        s_live[warp][stage] = live ? 0xffffu >> (TILE - min(left, TILE)) : 0;
+        mbar_expect_tx(bar, live ? S::STAGE : 0);
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < S::BOXES; ++c) load_box(to + c * S::BOX, &k_map, c * 64, head, in, from, bar);
+#pragma unroll
+          for (int c = 0; c < S::BOXES; ++c) load_box(to + S::ROWS + c * S::BOX, &v_map, c * 64, head, in, from, bar);
+        }
+      }
+    } else {
+      const bool is_v = lane >= 16;
+      const pla_b200_page_strides st = is_v ? p.v_strides : p.k_strides;
+      const act_t* src = static_cast<const act_t*>(p.q);            // a valid address for rows that are not read
+      if (live) src = static_cast<const act_t*>(is_v ? p.v_cache : p.k_cache) + from * st.block + in * st.token + head * st.head;
+      const uint32_t rows = __ballot_sync(0xffffffffu, live);
+      if (lane == 0) s_live[warp][stage] = rows & 0xffffu;
+#pragma unroll 4
+      for (int i = lane; i < 2 * TILE * (D / 8); i += 32) {
+        const int r = i / (D / 8), c = i % (D / 8);               // r: the lane that knows the row
+        const act_t* at_row = reinterpret_cast<const act_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r));
+        copy16(to + (r >> 4) * S::ROWS + (c >> 3) * S::BOX + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4), at_row + c * 8, (rows >> r) & 1);
+      }
+      copies_arrive(bar);
     }
     __syncwarp();
-    if (live) bulk_load(dst, src, D * 2, &s_full[warp][stage]);
   };
   for (int i = 0; i < min(STAGES, count); ++i) issue(i);
 
@@ -351,15 +391,21 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(c
     const int stage = i % STAGES;
     if (!timed_out) timed_out = __any_sync(0xffffffffu, !mbar_wait(&s_full[warp][stage], (i / STAGES) & 1));
     const uint32_t live = s_live[warp][stage];
-    const uint32_t k_rows = smem_addr(ring + stage * S::STAGE), v_rows = k_rows + S::ROWS;
+    const uint32_t k_rows = ring_addr + stage * S::STAGE, v_rows = k_rows + S::ROWS;
     if (live != 0 && !timed_out) {
+      if (BOXED && live != 0xffffu) {      // rows of the page past the request's end: p = 0 there, but 0 * garbage need not be 0
+        for (int i = lane; i < S::ROWS / 16; i += 32)
+          if (!((live >> ((i >> 3) & 15)) & 1)) reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::ROWS)[i] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+      }
       // scores of 16 tokens: lane holds tokens lane / 4 and + 8, heads 2 (lane % 4) and + 1
       float s[NT][2][4] = {};
-      const uint32_t ka = k_rows + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
+      const uint32_t ka = k_rows + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t a[4];
-        ldmatrix4(a, ka + kk * 32);
+        ldmatrix4(a, ka + (kk / 4) * S::BOX + ((((kk % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma<act_t>(s[n][kk & 1], a, qf[kk][n]);
       }
@@ -413,11 +459,11 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::CTAS) paged_decode_kernel(c
         pf[n][0] = transpose8x8(pack2<act_t>(c[0], c[1]));
         pf[n][1] = transpose8x8(pack2<act_t>(c[2], c[3]));
       }
-      const uint32_t va = v_rows + ((lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+      const uint32_t va = v_rows + ((lane & 7) + (lane >> 4) * 8) * 128;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t a[4];
-        ldmatrix4_trans(a, va + kk * 32);
+        ldmatrix4_trans(a, va + (kk / 4) * S::BOX + ((((kk % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma<act_t>(o[kk][n], a, pf[n]);
       }
@@ -518,14 +564,48 @@ int64_t workspace_bytes(int grid, int NT, int D) {
   return static_cast<int64_t>(grid) * sizeof(int4) + static_cast<int64_t>(2 * grid) * 8 * NT * (D + 2) * 4;
 }
 
-template <typename act_t, int D, int NT>
+// Tensor map of one cache: [page][token][head][channel], boxes of TILE tokens and 64 channels of one head. Axes of one entry get
+// any valid stride: their index is always 0.
+int cache_map(CUtensorMap* map, const pla_b200_paged_decode_args& a, void* base, const pla_b200_page_strides& st) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<void*> found{nullptr};
+  void* fn = found.load(std::memory_order_acquire);
+  if (fn == nullptr) {
+    cudaDriverEntryPointQueryResult how;
+    PLA_CUDA_OK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &how));
+    PLA_REQUIRE(fn != nullptr && how == cudaDriverEntryPointSuccess, PLA_B200_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    found.store(fn, std::memory_order_release);
+  }
+  auto bytes = [&](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(n <= 1 ? a.D : stride) * 2; };
+  const cuuint64_t size[4] = {static_cast<cuuint64_t>(a.D), static_cast<cuuint64_t>(a.Hk), static_cast<cuuint64_t>(a.block_size),
+                              static_cast<cuuint64_t>(a.num_blocks)};
+  const cuuint64_t stride[3] = {bytes(a.Hk, st.head), bytes(a.block_size, st.token), bytes(a.num_blocks, st.block)};
+  const cuuint32_t box[4] = {64, 1, TILE, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult rc = reinterpret_cast<Encode>(fn)(
+      map, a.act_dtype == PLA_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, size, stride, box, step,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  PLA_REQUIRE(rc == CUDA_SUCCESS, PLA_B200_E_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(rc));
+  return PLA_B200_OK;
+}
+
+// Strides that a tensor map can hold; pages of whole tiles.
+bool boxed(const pla_b200_paged_decode_args& a) {
+  auto fits = [&](const pla_b200_page_strides& s) {
+    auto ok = [](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride < int64_t{1} << 38); };
+    return ok(a.num_blocks, s.block) && ok(a.block_size, s.token) && ok(a.Hk, s.head);
+  };
+  return a.block_size % TILE == 0 && a.num_blocks > 0 && a.num_blocks <= INT32_MAX && fits(a.k_strides) && fits(a.v_strides);
+}
+
+template <typename act_t, int D, int NT, bool BOXED>
 int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   using S = Shape<D>;
   static DeviceOnce once;
   int dev = 0;
   PLA_CUDA_OK(cudaGetDevice(&dev));
   if (once.needed(dev)) {
-    PLA_CUDA_OK(cudaFuncSetAttribute(paged_decode_kernel<act_t, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    PLA_CUDA_OK(cudaFuncSetAttribute(paged_decode_kernel<act_t, D, NT, BOXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     once.mark(dev);
   }
   Plan plan;
@@ -541,7 +621,13 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   plan.part_m = plan.part_o + static_cast<int64_t>(2 * plan.grid) * 8 * NT * D;
   plan.part_l = plan.part_m + static_cast<int64_t>(2 * plan.grid) * 8 * NT;
   PLA_REQUIRE(a.workspace_bytes >= workspace_bytes(plan.grid, NT, D), PLA_B200_E_INVALID, "the workspace is too small");
-  paged_decode_kernel<act_t, D, NT><<<plan.grid, THREADS, S::SMEM, stream>>>(a, plan);
+  CUtensorMap k_map = {}, v_map = {};
+  if constexpr (BOXED) {
+    int rc = cache_map(&k_map, a, const_cast<void*>(a.k_cache), a.k_strides);
+    if (rc == PLA_B200_OK) rc = cache_map(&v_map, a, const_cast<void*>(a.v_cache), a.v_strides);
+    if (rc != PLA_B200_OK) return rc;
+  }
+  paged_decode_kernel<act_t, D, NT, BOXED><<<plan.grid, THREADS, S::SMEM, stream>>>(a, plan, k_map, v_map);
   PLA_CUDA_OK(cudaGetLastError());
   if (per_item > 1) {                               // else every item is one unit and was stored whole
     cudaLaunchConfig_t cfg = {};
@@ -558,15 +644,21 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   return PLA_B200_OK;
 }
 
+template <typename act_t, int D>
+int launch_size(const pla_b200_paged_decode_args& a, cudaStream_t s) {
+  const bool one = tiles_of(a.Hq / a.Hk) == 1;
+  if (boxed(a)) return one ? launch<act_t, D, 1, true>(a, s) : launch<act_t, D, 2, true>(a, s);
+  return one ? launch<act_t, D, 1, false>(a, s) : launch<act_t, D, 2, false>(a, s);
+}
+
 template <typename act_t>
 int launch_for(const pla_b200_paged_decode_args& a, cudaStream_t s) {
-  const bool one = tiles_of(a.Hq / a.Hk) == 1;
   switch (a.D) {
-    case 64: return one ? launch<act_t, 64, 1>(a, s) : launch<act_t, 64, 2>(a, s);
-    case 96: return one ? launch<act_t, 96, 1>(a, s) : launch<act_t, 96, 2>(a, s);
-    case 128: return one ? launch<act_t, 128, 1>(a, s) : launch<act_t, 128, 2>(a, s);
-    case 192: return one ? launch<act_t, 192, 1>(a, s) : launch<act_t, 192, 2>(a, s);
-    default: return one ? launch<act_t, 256, 1>(a, s) : launch<act_t, 256, 2>(a, s);
+    case 64: return launch_size<act_t, 64>(a, s);
+    case 96: return launch_size<act_t, 96>(a, s);
+    case 128: return launch_size<act_t, 128>(a, s);
+    case 192: return launch_size<act_t, 192>(a, s);
+    default: return launch_size<act_t, 256>(a, s);
   }
 }
 
