@@ -9,12 +9,13 @@
 //
 // Work: units of 64 tokens of one (request, key/value head). Every CTA adds up the lengths itself and takes an equal, consecutive
 // range of all units (the lengths are on the device, so the host could not split them), which keeps the SMs equally loaded whatever
-// the lengths are and splits a single long request over all of them. In a unit each of the four warps takes 16 tokens, keeps its own
-// maxima, sums and output, and streams its rows through its own ring of shared memory, without a barrier between warps until the
-// range leaves the (request, head). Where pages hold whole tiles of 16 tokens, a tile is a box of a tensor map over the cache and one
-// lane brings it with a copy per 64 channels; other page sizes take 16-byte asynchronous copies from each row's page. (One bulk copy
-// per row and lane was tried first: the 32 lanes' copies issue one after another, 480 of 620 instructions per tile; 256 us where
-// the boxes take XXX for 64 requests up to 16K tokens of D = 256.) Both leave the 128-byte swizzle that ldmatrix reads without bank conflicts.
+// the lengths are and splits a single long request over all of them. A producer warp walks the range and keeps a ring of units in
+// shared memory filled; in a unit each of the four other warps takes 16 tokens and keeps its own maxima, sums and output, without a
+// barrier between them until the range leaves the (request, head). Where pages hold whole tiles of 16 tokens, a tile is a box of a
+// tensor map over the cache, one copy per 64 channels; other page sizes take 16-byte asynchronous copies from each row's page. Both
+// leave the 128-byte swizzle that ldmatrix reads without bank conflicts. Tried before: one bulk copy per row and lane (the lanes'
+// copies issue one after another, 480 of 620 instructions per tile) and every warp loading for itself (240 instructions per tile
+// where this takes XXX; shorter heads and contexts are bound by them).
 // A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
 // waits on the first one's end only, joins the parts in order: no atomics, the same bits every time.
 // Scores, sums and outputs are 32-bit; the weights p are rounded to the activations' type for the product with V (relative 2^-8
@@ -28,37 +29,51 @@ namespace pla {
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int THREADS = WARPS * 32;
+constexpr int THREADS = WARPS * 32;   // of the warps that compute; one more loads
 constexpr int TILE = 16;              // tokens per warp and step
 constexpr int UNIT = TILE * WARPS;    // tokens per CTA and step
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float SLACK = 8.0f;         // the running maximum may lag this far (log2) behind: p stays below 2^8, fewer rescalings
 
-// Ring depth per warp, and CTAs per SM that its shared memory leaves room for (of 227 KB): at least 96 KB in flight per SM.
+// Ring depth, and CTAs per SM that its shared memory leaves room for (of 227 KB): 192 KB of rows in flight per SM.
 template <int D>
 struct Shape {
-  static constexpr int BOXES = (D + 63) / 64;              // 64 channels of 16 rows each: 2 KB
-  static constexpr int BOX = TILE * 128;
-  static constexpr int ROWS = BOXES * BOX;                 // keys (or values) of a tile
+  static constexpr int BOXES = (D + 63) / 64;              // 64 channels of a unit's rows, 128 bytes each
+  static constexpr int BOX = UNIT * 128;
+  static constexpr int ROWS = BOXES * BOX;                 // keys (or values) of a unit
   static constexpr int STAGE = 2 * ROWS;
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int CTAS = D > 128 ? 1 : D > 64 ? 2 : 3;
+  static constexpr int STAGES = 192 * 1024 / CTAS / STAGE;
   static constexpr int HALF = D / 2;
   static constexpr int OP = HALF + 4;                      // row pitch (floats) of the join buffer
   static constexpr int JOIN = WARPS * 8 * OP * 4;
-  static constexpr int SMEM = 1024 + RING + JOIN;          // the ring begins at a multiple of 1,024 bytes
-  static constexpr int CTAS = SMEM > 113 * 1024 ? 1 : SMEM > 75 * 1024 ? 2 : 3;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + JOIN;   // the ring begins at a multiple of 1,024 bytes
+};
+
+// Division of numbers below 2^31 by a fixed d: (t * m) >> (31 + L) with L = ceil(log2 d), m = floor(2^(31 + L) / d) + 1, exact because
+// m d exceeds 2^(31 + L) by at most d <= 2^L.
+struct Divisor {
+  uint32_t d, m, shift;
+  explicit Divisor(uint32_t by = 1) : d(by), shift(31) {
+    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
+    m = static_cast<uint32_t>((uint64_t{1} << shift) / d + 1);
+  }
+  __device__ __forceinline__ int quotient(int t) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * m) >> shift);
+  }
 };
 
 struct Plan {              // of one call, the same on host and device
+  Divisor page;            // by block_size
   int chunks;              // groups of 8 * NT query heads per key/value head
   int group;               // query heads per key/value head
   int grid;
   float* part_o;           // [2 * grid][8 * NT][D]
   float* part_m;           // [2 * grid][8 * NT]
   float* part_l;
-  int4* head_part;         // [grid]: {request, head item, last CTA that holds a part of it, 1}; w = 0: nothing begins here and goes on
+  int4* spans;             // [2 * grid]: the split item that CTA i goes on with (2 i), the one that begins in it (2 i + 1):
+                           // {request, item, first CTA, last CTA}, last = -1: none
 };
 
 template <typename act_t>
@@ -127,16 +142,18 @@ __device__ __forceinline__ int length_of(const pla_b200_paged_decode_args& p, in
   return n < 0 ? 0 : n > room ? static_cast<int>(room) : n;
 }
 
-// A place in the sequence of units: request, (key/value head, chunk) item of it, unit of the item.
+// A place in the sequence of units: request, its item (key/value head and chunk of its query heads), unit of the item.
 struct Place {
-  int b, item, unit, units, len;
+  int b, head, chunk, unit, units, len;
 };
 
-__device__ __forceinline__ void advance(Place& x, const pla_b200_paged_decode_args& p, int items) {
+__device__ __forceinline__ void advance(Place& x, const pla_b200_paged_decode_args& p, int chunks) {
   if (++x.unit < x.units) return;
   x.unit = 0;
-  if (++x.item < items) return;
-  x.item = 0;
+  if (++x.chunk < chunks) return;
+  x.chunk = 0;
+  if (++x.head < p.Hk) return;
+  x.head = 0;
   int32_t ignored = 0;
   do {
     if (++x.b >= p.B) {                 // past the end: the caller counts its units and never uses this place
@@ -149,22 +166,28 @@ __device__ __forceinline__ void advance(Place& x, const pla_b200_paged_decode_ar
   } while (x.units == 0);
 }
 
+// Barrier of the warps that compute.
+__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
 // BOXED: pages hold whole tiles, the maps describe the caches.
 template <typename act_t, int D, int NT, bool BOXED>
-__global__ void __launch_bounds__(THREADS, Shape<D>::CTAS)
+__global__ void __launch_bounds__(THREADS + 32, Shape<D>::CTAS)
 paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D>;
   constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
-  __shared__ uint64_t s_full[WARPS][STAGES];
-  __shared__ uint32_t s_live[WARPS][STAGES];
+  __shared__ uint64_t s_full[STAGES], s_free[STAGES];
+  __shared__ uint16_t s_live[STAGES][WARPS];       // rows of each tile that hold a token
   __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
-  __shared__ int64_t s_scan[WARPS];
-  __shared__ int64_t s_total;
-  __shared__ int s_place[3];
+  __shared__ int64_t s_scan[WARPS + 1];
+  __shared__ int s_place[4];
   asm volatile("griddepcontrol.launch_dependents;");
+  if (BOXED && threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+  }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int items = p.Hk * plan.chunks;
   int32_t bad = 0;
@@ -182,28 +205,35 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
     if (lane >= o) upto += x;
   }
   if (lane == 31) s_scan[warp] = upto;
-  if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&s_full[warp][i], BOXED ? 1 : 32);
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s_full[i], BOXED ? 1 : 33);       // the producer's lane 0, and every lane's copies
+      mbar_init(&s_free[i], WARPS);
+    }
     fence_mbar_init();
   }
   __syncthreads();
   int64_t total = 0;
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w <= WARPS; ++w) {
     if (w < warp) upto += s_scan[w];
     total += s_scan[w];
   }
-  // requests of length zero are nobody's unit
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    int32_t ignored = 0;
-    if (length_of(p, b, ignored) != 0) continue;
-    act_t* o = static_cast<act_t*>(p.out) + static_cast<int64_t>(b) * p.Hq * D;
-    for (int i = tid; i < p.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
-    if (p.lse != nullptr)
-      for (int i = tid; i < p.Hq; i += THREADS) p.lse[static_cast<int64_t>(b) * p.Hq + i] = -INFINITY;
-  }
   const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
+  // Requests of length zero are nobody's unit.
+  auto clear_empty = [&] {
+    if (tid >= THREADS) return;
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+      int32_t ignored = 0;
+      if (length_of(p, b, ignored) != 0) continue;
+      act_t* out = static_cast<act_t*>(p.out) + static_cast<int64_t>(b) * p.Hq * D;
+      for (int i = tid; i < p.Hq * D / 8; i += THREADS) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+      if (p.lse != nullptr)
+        for (int i = tid; i < p.Hq; i += THREADS) p.lse[static_cast<int64_t>(b) * p.Hq + i] = -INFINITY;
+    }
+  };
   if (blockIdx.x >= workers) {
-    if (tid == 0) plan.head_part[blockIdx.x] = make_int4(0, 0, 0, 0);
+    clear_empty();
+    if (tid < 2) plan.spans[2 * blockIdx.x + tid] = make_int4(0, 0, 0, -1);
     if (blockIdx.x == 0 && bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
     return;
   }
@@ -217,6 +247,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
         s_place[0] = b;
         s_place[1] = static_cast<int>(left / units);
         s_place[2] = static_cast<int>(left % units);
+        s_place[3] = length_of(p, b, ignored);
         break;
       }
       left -= units * items;
@@ -225,76 +256,98 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
   __syncthreads();
   Place at;
   at.b = s_place[0];
-  at.item = s_place[1];
+  at.head = s_place[1] / plan.chunks;
+  at.chunk = s_place[1] % plan.chunks;
   at.unit = s_place[2];
-  {
-    int32_t ignored = 0;
-    at.len = length_of(p, at.b, ignored);
-    at.units = (at.len + UNIT - 1) / UNIT;
-  }
+  at.len = s_place[3];
+  at.units = (at.len + UNIT - 1) / UNIT;
   const int count = static_cast<int>(end - begin);
 
-  // ---- loads
-  uint8_t* ring = smem + warp * (STAGES * S::STAGE);
-  const uint32_t ring_addr = smem_addr(ring);
-  Place ahead = at;
-  int issued = 0;
-  // The lane's token of the tile: all lanes the first one's when it comes as a box, else lanes r and r + 16 row r's (keys and values).
-  const int row = BOXED ? 0 : lane & 15;
-  auto page_of = [&](const Place& x) -> int {     // -1 past the end
-    const int t = x.unit * UNIT + warp * TILE + row;
-    return t < x.len ? p.block_table[x.b * p.table_row_stride + t / p.block_size] : -1;
-  };
-  int page = page_of(ahead);
-  auto issue = [&](int stage) {
-    const int t = ahead.unit * UNIT + warp * TILE + row, in = t % p.block_size, head = ahead.item / plan.chunks, left = ahead.len - t;
-    const bool live = left > 0 && page >= 0 && page < p.num_blocks;
-    if (left > 0 && !live) bad |= PLA_B200_DEV_BAD_SLOT;
-    const uint32_t to = ring_addr + stage * S::STAGE;
-    uint64_t* const bar = &s_full[warp][stage];
-    const int from = page;
-    ++issued;
-    if (issued < count) {
-      advance(ahead, p, items);
-      page = page_of(ahead);                      // used one step later
-    }
-    if constexpr (BOXED) {
-      if (lane == 0) {
-        s_live[warp][stage] = live ? 0xffffu >> (TILE - min(left, TILE)) : 0;
-        mbar_expect_tx(bar, live ? S::STAGE : 0);
-        if (live) {
+  const uint32_t ring = smem_addr(smem);
+  bool timed_out = false;
+  if (warp == WARPS) {
+    // ---- producer: token of the lane, that of tile lane % 4 when tiles come as boxes, else those of rows lane and lane + 32
+    auto page_of = [&](int t) -> int {               // -1 past the end
+      return t < at.len ? p.block_table[at.b * p.table_row_stride + plan.page.quotient(t)] : -1;
+    };
+    constexpr int TOKENS = BOXED ? 1 : 2;
+    auto token = [&](int u) { return at.unit * UNIT + (BOXED ? (lane & 3) * TILE : lane + u * 32); };
+    int page[TOKENS];
 #pragma unroll
-          for (int c = 0; c < S::BOXES; ++c) load_box(to + c * S::BOX, &k_map, c * 64, head, in, from, bar);
+    for (int u = 0; u < TOKENS; ++u) page[u] = page_of(token(u));
+    for (int i = 0; i < count; ++i) {
+      const int stage = i % STAGES, head = at.head;
+      if (i >= STAGES) timed_out = __any_sync(0xffffffffu, !mbar_wait(&s_free[stage], (i / STAGES - 1) & 1));
+      if (timed_out) break;
+      int left[TOKENS], in[TOKENS], from[TOKENS];
+      bool live[TOKENS];
 #pragma unroll
-          for (int c = 0; c < S::BOXES; ++c) load_box(to + S::ROWS + c * S::BOX, &v_map, c * 64, head, in, from, bar);
+      for (int u = 0; u < TOKENS; ++u) {
+        const int t = token(u);
+        left[u] = at.len - t;
+        in[u] = t - plan.page.quotient(t) * p.block_size;
+        from[u] = page[u];
+        live[u] = left[u] > 0 && page[u] >= 0 && page[u] < p.num_blocks;
+        if (left[u] > 0 && !live[u]) bad |= PLA_B200_DEV_BAD_SLOT;
+      }
+      if (i + 1 < count) {
+        advance(at, p, plan.chunks);
+#pragma unroll
+        for (int u = 0; u < TOKENS; ++u) page[u] = page_of(token(u));      // used one step later
+      }
+      const uint32_t to = ring + stage * S::STAGE;
+      uint64_t* const bar = &s_full[stage];
+      if constexpr (BOXED) {
+        if (lane < WARPS) s_live[stage][lane] = live[0] ? 0xffffu >> (TILE - min(left[0], TILE)) : 0;
+        const uint32_t tiles = __ballot_sync(0xffffffffu, live[0]) & 0xfu;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(bar, __popc(tiles) * (2 * S::BOXES * TILE * 128));
+        __syncwarp();
+        if (lane < WARPS && live[0]) {
+          const uint32_t row = to + lane * (TILE * 128);
+#pragma unroll
+          for (int c = 0; c < S::BOXES; ++c) load_box(row + c * S::BOX, &k_map, c * 64, head, in[0], from[0], bar);
+#pragma unroll
+          for (int c = 0; c < S::BOXES; ++c) load_box(row + S::ROWS + c * S::BOX, &v_map, c * 64, head, in[0], from[0], bar);
         }
-      }
-    } else {
-      const bool is_v = lane >= 16;
-      const pla_b200_page_strides st = is_v ? p.v_strides : p.k_strides;
-      const act_t* src = static_cast<const act_t*>(p.q);            // a valid address for rows that are not read
-      if (live) src = static_cast<const act_t*>(is_v ? p.v_cache : p.k_cache) + from * st.block + in * st.token + head * st.head;
-      const uint32_t rows = __ballot_sync(0xffffffffu, live);
-      if (lane == 0) s_live[warp][stage] = rows & 0xffffu;
+      } else {
+        uint32_t rows[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) rows[u] = __ballot_sync(0xffffffffu, live[u]);
+        if (lane < WARPS) s_live[stage][lane] = static_cast<uint16_t>(rows[lane >> 1] >> ((lane & 1) * 16));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {                            // keys, values
+          const pla_b200_page_strides st = side ? p.v_strides : p.k_strides;
+          const act_t* const base = static_cast<const act_t*>(side ? p.v_cache : p.k_cache);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const act_t* src = static_cast<const act_t*>(p.q);            // a valid address for rows that are not read
+            if (live[u]) src = base + from[u] * st.block + in[u] * st.token + head * st.head;
 #pragma unroll 4
-      for (int i = lane; i < 2 * TILE * (D / 8); i += 32) {
-        const int r = i / (D / 8), c = i % (D / 8);               // r: the lane that knows the row
-        const act_t* at_row = reinterpret_cast<const act_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r));
-        copy16(to + (r >> 4) * S::ROWS + (c >> 3) * S::BOX + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4), at_row + c * 8, (rows >> r) & 1);
+            for (int k = lane; k < 32 * (D / 8); k += 32) {
+              const int r = k / (D / 8), c = k % (D / 8);                 // r: the lane that knows the row
+              const act_t* row = reinterpret_cast<const act_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r));
+              copy16(to + side * S::ROWS + (c >> 3) * S::BOX + (u * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), row + c * 8, (rows[u] >> r) & 1);
+            }
+          }
+        }
+        copies_arrive(bar);
       }
-      copies_arrive(bar);
     }
-    __syncwarp();
-  };
-  for (int i = 0; i < min(STAGES, count); ++i) issue(i);
+    if (timed_out) bad |= PLA_B200_DEV_WAIT_TIMEOUT;
+    if (bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
+    return;
+  }
+  clear_empty();
 
   // ---- the lane's part of the running state: heads 2 (lane % 4) and the next of each group of eight
   float m[NT][2], l[NT][2], o[D / 16][NT][4];
   uint32_t qf[D / 16][NT][2];
   const float to_log2 = p.scale * LOG2E;
   auto load_q = [&](const Place& x) {
-    const int chunk = x.item % plan.chunks, head = (x.item / plan.chunks) * plan.group + chunk * 8 * NT;
-    const int heads = min(8 * NT, plan.group - chunk * 8 * NT);
+    const int head = x.head * plan.group + x.chunk * 8 * NT, heads = min(8 * NT, plan.group - x.chunk * 8 * NT);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int h = n * 8 + lane / 4;
@@ -318,10 +371,10 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
     }
   };
 
-  // Joins the four warps' parts of the item that ends here (or leaves the range) and stores them.
+  // Joins the four warps' parts of the item that ends here (or leaves the range) and stores them: as output, or as a part.
   auto flush = [&](const Place& x, bool whole, int slot) {
-    const int chunk = x.item % plan.chunks, head = (x.item / plan.chunks) * plan.group + chunk * 8 * NT;
-    const int heads = min(8 * NT, plan.group - chunk * 8 * NT);
+    const int head = x.head * plan.group + x.chunk * 8 * NT, heads = min(8 * NT, plan.group - x.chunk * 8 * NT);
+    const int64_t first_row = static_cast<int64_t>(x.b) * p.Hq + head, first_part = static_cast<int64_t>(slot) * 8 * NT;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -333,16 +386,29 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           s_l[warp][n * 8 + lane * 2 + i] = l[n][i];
         }
       }
-    __syncthreads();
-    float* join = reinterpret_cast<float*>(smem + S::RING);
+    compute_barrier();
+    float* join = reinterpret_cast<float*>(smem + STAGES * S::STAGE);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float down[2];
+      float down[2];                       // what the lane's two heads are multiplied by
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float top = -INFINITY;
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][n * 8 + (lane % 4) * 2 + i]);
+        const int h = n * 8 + (lane % 4) * 2 + i;
+        float top = -INFINITY, weight = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][h]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) weight += s_m[w][h] == -INFINITY ? 0.0f : s_l[w][h] * fast_exp2(s_m[w][h] - top);
         down[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - top);
+        if (whole) down[i] = weight == 0.0f ? 0.0f : down[i] / weight;
+        if (warp == 0 && lane < 4 && h < heads) {
+          if (!whole) {
+            plan.part_m[first_part + h] = top;
+            plan.part_l[first_part + h] = weight;
+          } else if (p.lse != nullptr) {
+            p.lse[first_row + h] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
+          }
+        }
       }
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
@@ -356,46 +422,49 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           to[8] = c[2] * down[0];
           to[S::OP + 8] = c[3] * down[1];
         }
-        __syncthreads();
-        for (int i = tid; i < 8 * S::HALF; i += THREADS) {
-          const int h = i / S::HALF, d = i % S::HALF, hh = n * 8 + h;
-          if (hh >= heads) continue;
-          float sum = 0.0f;
+        compute_barrier();
 #pragma unroll
-          for (int w = 0; w < WARPS; ++w) sum += join[(w * 8 + h) * S::OP + d];
-          float top = -INFINITY, weight = 0.0f;
-          for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][hh]);
-          for (int w = 0; w < WARPS; ++w) weight += s_m[w][hh] == -INFINITY ? 0.0f : s_l[w][hh] * fast_exp2(s_m[w][hh] - top);
-          const bool first = part == 0 && d == 0;
-          if (whole) {
-            const int64_t out = static_cast<int64_t>(x.b) * p.Hq + head + hh;
-            static_cast<act_t*>(p.out)[out * D + part * S::HALF + d] = from_f32<act_t>(weight == 0.0f ? 0.0f : sum / weight);
-            if (first && p.lse != nullptr) p.lse[out] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
-          } else {
-            const int64_t to = static_cast<int64_t>(slot) * 8 * NT + hh;
-            plan.part_o[to * D + part * S::HALF + d] = sum;
-            if (first) plan.part_m[to] = top, plan.part_l[to] = weight;
+        for (int i = tid; i < 2 * S::HALF; i += THREADS) {       // four channels of a head
+          const int h = i / (S::HALF / 4), d = i % (S::HALF / 4) * 4, hh = n * 8 + h;
+          if (hh >= heads) continue;
+          float4 sum = *reinterpret_cast<const float4*>(join + h * S::OP + d);
+#pragma unroll
+          for (int w = 1; w < WARPS; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + h) * S::OP + d);
+            sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
           }
+          if (whole)
+            *reinterpret_cast<uint2*>(static_cast<act_t*>(p.out) + (first_row + hh) * D + part * S::HALF + d) =
+                make_uint2(pack2<act_t>(sum.x, sum.y), pack2<act_t>(sum.z, sum.w));
+          else
+            *reinterpret_cast<float4*>(plan.part_o + (first_part + hh) * D + part * S::HALF + d) = sum;
         }
-        __syncthreads();
+        if (part == 0 || n + 1 < NT) compute_barrier();            // the buffer is written again
       }
     }
   };
 
-  int4 begins = make_int4(0, 0, 0, 0);
+  // The CTA that holds unit u.
+  auto holder = [&](int64_t u) { return static_cast<int>(((u + 1) * workers - 1) / total); };
   int first_unit = at.unit;
+  int4 goes_on = make_int4(0, 0, 0, -1), begins = make_int4(0, 0, 0, -1);
+  if (first_unit > 0) goes_on = make_int4(at.b, at.head * plan.chunks + at.chunk, holder(begin - first_unit), holder(begin + at.units - 1 - first_unit));
   clear();
   load_q(at);
-  bool timed_out = false;
+  int late = 0;
   for (int i = 0; i < count; ++i) {
     const int stage = i % STAGES;
-    if (!timed_out) timed_out = __any_sync(0xffffffffu, !mbar_wait(&s_full[warp][stage], (i / STAGES) & 1));
-    const uint32_t live = s_live[warp][stage];
-    const uint32_t k_rows = ring_addr + stage * S::STAGE, v_rows = k_rows + S::ROWS;
+    if (!timed_out && __any_sync(0xffffffffu, !mbar_wait(&s_full[stage], (i / STAGES) & 1))) {
+      timed_out = true;
+      late = i;
+    }
+    const uint32_t live = s_live[stage][warp];
+    const uint32_t k_rows = ring + stage * S::STAGE + warp * (TILE * 128), v_rows = k_rows + S::ROWS;
     if (live != 0 && !timed_out) {
       if (BOXED && live != 0xffffu) {      // rows of the page past the request's end: p = 0 there, but 0 * garbage need not be 0
-        for (int i = lane; i < S::ROWS / 16; i += 32)
-          if (!((live >> ((i >> 3) & 15)) & 1)) reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::ROWS)[i] = make_uint4(0, 0, 0, 0);
+        for (int k = lane; k < S::BOXES * TILE * 8; k += 32)
+          if (!((live >> ((k >> 3) & 15)) & 1))
+            *reinterpret_cast<uint4*>(smem + (v_rows - ring) + (k >> 7) * S::BOX + (k & 127) * 16) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
         __syncwarp();
       }
@@ -409,7 +478,6 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma<act_t>(s[n][kk & 1], a, qf[kk][n]);
       }
-      const bool on0 = (live >> (lane / 4)) & 1, on1 = (live >> (lane / 4 + 8)) & 1;
       uint32_t pf[NT][2];
       float next[NT][2];
       bool grow = false;
@@ -417,7 +485,12 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
       for (int n = 0; n < NT; ++n) {
         float* c = s[n][0];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = (e < 2 ? on0 : on1) ? (c[e] + s[n][1][e]) * to_log2 : -INFINITY;
+        for (int e = 0; e < 4; ++e) c[e] = (c[e] + s[n][1][e]) * to_log2;
+        if (live != 0xffffu) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!((live >> (lane / 4 + (e < 2 ? 0 : 8))) & 1)) c[e] = -INFINITY;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float x = fmaxf(c[e], c[e + 2]);
@@ -469,86 +542,118 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
       }
     }
     __syncwarp();
-    if (issued < count && !timed_out) issue(stage);
+    if (lane == 0) mbar_arrive(&s_free[stage]);
     if (at.unit + 1 == at.units || i + 1 == count) {
       const bool whole = first_unit == 0 && at.unit + 1 == at.units;
-      if (first_unit == 0 && !whole) {
-        // this part begins the item: name the last CTA that goes on with it
-        const int64_t item_end = end + (at.units - 1 - at.unit);
-        begins = make_int4(at.b, at.item, static_cast<int>((item_end * workers - 1) / total), 1);
-      }
-      flush(at, whole, 2 * blockIdx.x + (first_unit == 0 ? 1 : 0));
+      const int slot = 2 * blockIdx.x + (first_unit == 0 ? 1 : 0);
+      if (first_unit == 0 && !whole) begins = make_int4(at.b, at.head * plan.chunks + at.chunk, blockIdx.x, holder(end + at.units - 2 - at.unit));
+      const Place done = at;
+      advance(at, p, plan.chunks);
+      if (i + 1 < count) load_q(at);          // arrives while the parts are joined
+      flush(done, whole, slot);
       clear();
       first_unit = 0;
-      const int item = at.item, b = at.b;
-      advance(at, p, items);
-      if (i + 1 < count && (item != at.item || b != at.b)) load_q(at);
     } else {
       ++at.unit;
     }
   }
-  if (timed_out) {                       // a copy never came: say so, and give the others time to land before the CTA's memory goes
+  if (timed_out) {               // a copy never came: say so, and give those in flight time to land before the CTA's memory goes
     bad |= PLA_B200_DEV_WAIT_TIMEOUT;
-    for (int i = max(issued - STAGES, 0); i < issued; ++i) mbar_wait(&s_full[warp][i % STAGES], (i / STAGES) & 1);
+    for (int i = late; i < min(late + STAGES, count); ++i) mbar_wait(&s_full[i % STAGES], (i / STAGES) & 1);
   }
-  if (tid == 0) plan.head_part[blockIdx.x] = begins;
+  if (tid == 0) {
+    plan.spans[2 * blockIdx.x] = goes_on;
+    plan.spans[2 * blockIdx.x + 1] = begins;
+  }
   if (bad != 0 && p.status != nullptr) atomicOr(p.status, bad);
 }
 
-// Joins the parts of every item that lies in several CTAs' ranges: CTA (i, h) that of the item which begins in the range of CTA i, head h.
+// Joins the parts of every item that lies in several CTAs' ranges; CTA 2 i does the item that main CTA i goes on with, CTA 2 i + 1 the
+// one that begins there. The CTAs of an item share its heads: the j-th of n takes heads j, j + n, ...; a head's parts are spread
+// over the warps, a lane holds four channels of every 128. Small on purpose: its instructions come from memory, not from a warm cache.
+constexpr int JOIN_WARPS = 8, AT_ONCE = 4;
+
 template <typename act_t, int D, int NT>
-__global__ void __launch_bounds__(THREADS) paged_join_kernel(const pla_b200_paged_decode_args p, const Plan plan) {
-  constexpr int VEC = D / 4, GROUPS = THREADS / VEC;     // threads per part, parts read at a time
-  __shared__ float s_red[WARPS];
-  __shared__ float4 s_o[GROUPS][VEC];
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const pla_b200_paged_decode_args p, const Plan plan) {
+  constexpr int C = (D + 127) / 128;
+  __shared__ float s_m[JOIN_WARPS], s_l[JOIN_WARPS];
+  __shared__ float4 s_o[JOIN_WARPS][D / 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 begins = plan.head_part[blockIdx.x];
-  if (begins.w == 0) return;
-  const int chunk = begins.y % plan.chunks, h = blockIdx.y;
-  if (h >= min(8 * NT, plan.group - chunk * 8 * NT)) return;
-  const int i = blockIdx.x, parts = begins.z - i + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto index = [&](int j) -> int64_t { return static_cast<int64_t>(j == 0 ? 2 * i + 1 : 2 * (i + j)) * 8 * NT + h; };
-  float top = -INFINITY;
-  for (int j = tid; j < parts; j += THREADS) top = fmaxf(top, plan.part_m[index(j)]);
+  const int4 span = plan.spans[blockIdx.x];
+  if (span.w < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = span.y % plan.chunks, heads = min(8 * NT, plan.group - chunk * 8 * NT);
+  const int parts = span.w - span.z + 1, rank = blockIdx.x / 2 - span.z;
+  const int mine = rank < heads ? (heads - rank + parts - 1) / parts : 0;      // heads of this CTA: at most 8 of 16, as parts > 1
+  if (mine == 0) return;
+  int slices = JOIN_WARPS;                                                     // warps per head
+  while (slices * mine > JOIN_WARPS) slices >>= 1;
+  const int slot = warp / slices, slice = warp % slices, h = rank + slot * parts;
+  float top = -INFINITY, weight = 0.0f;
+  float4 sum[C] = {};
+  if (slot < mine) {
+    for (int j0 = slice; j0 < parts; j0 += AT_ONCE * slices) {
+      float m[AT_ONCE], l[AT_ONCE], next = top;
+      float4 x[AT_ONCE][C];
 #pragma unroll
-  for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-  if (lane == 0) s_red[warp] = top;
-  __syncthreads();
-  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_red[w]);
-  __syncthreads();
-  float weight = 0.0f;
-  for (int j = tid; j < parts; j += THREADS) {
-    const float m = plan.part_m[index(j)];
-    if (m != -INFINITY) weight += plan.part_l[index(j)] * fast_exp2(m - top);
-  }
-  weight = warp_sum(weight);
-  if (lane == 0) s_red[warp] = weight;
-  const int g = tid / VEC, d = tid % VEC;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (g < GROUPS) {
-    for (int j = g; j < parts; j += GROUPS) {
-      const float m = plan.part_m[index(j)];
-      const float f = m == -INFINITY ? 0.0f : fast_exp2(m - top);
-      const float4 x = reinterpret_cast<const float4*>(plan.part_o + index(j) * D)[d];
-      sum.x += x.x * f, sum.y += x.y * f, sum.z += x.z * f, sum.w += x.w * f;
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int j = j0 + u * slices;
+        const bool on = j < parts;
+        const int64_t at = static_cast<int64_t>(2 * (span.z + j) + (j == 0 ? 1 : 0)) * 8 * NT + h;
+        m[u] = on ? plan.part_m[at] : -INFINITY;
+        l[u] = on ? plan.part_l[at] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          x[u][c] = on && c * 32 + lane < D / 4 ? reinterpret_cast<const float4*>(plan.part_o + at * D)[c * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) next = fmaxf(next, m[u]);
+      const float base = next == -INFINITY ? 0.0f : next;       // exp2(-inf - base) = 0
+      const float down = fast_exp2(top - base);
+      top = next;
+      weight *= down;
+#pragma unroll
+      for (int c = 0; c < C; ++c) sum[c].x *= down, sum[c].y *= down, sum[c].z *= down, sum[c].w *= down;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const float f = fast_exp2(m[u] - base);
+        weight += l[u] * f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          sum[c].x += x[u][c].x * f, sum[c].y += x[u][c].y * f, sum[c].z += x[u][c].z * f, sum[c].w += x[u][c].w * f;
+      }
     }
-    s_o[g][d] = sum;
+    if (lane == 0) s_m[warp] = top, s_l[warp] = weight;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * 32 + lane < D / 4) s_o[warp][c * 32 + lane] = sum[c];
   }
   __syncthreads();
+  if (slot >= mine || slice != 0) return;
+  for (int k = 1; k < slices; ++k) top = fmaxf(top, s_m[warp + k]);
+  const float base = top == -INFINITY ? 0.0f : top;
   weight = 0.0f;
-  for (int w = 0; w < WARPS; ++w) weight += s_red[w];
-  if (tid < VEC) {
 #pragma unroll
-    for (int k = 1; k < GROUPS; ++k) {
-      const float4 x = s_o[k][tid];
-      sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-    }
-    const float f = weight == 0.0f ? 0.0f : 1.0f / weight;
-    const int64_t out = static_cast<int64_t>(begins.x) * p.Hq + (begins.y / plan.chunks) * plan.group + chunk * 8 * NT + h;
-    uint2 raw = make_uint2(pack2<act_t>(sum.x * f, sum.y * f), pack2<act_t>(sum.z * f, sum.w * f));
-    *reinterpret_cast<uint2*>(static_cast<act_t*>(p.out) + out * D + tid * 4) = raw;
-    if (tid == 0 && p.lse != nullptr) p.lse[out] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
+  for (int c = 0; c < C; ++c) sum[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+  for (int k = 0; k < slices; ++k) {
+    const float f = fast_exp2(s_m[warp + k] - base);
+    weight += s_l[warp + k] * f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * 32 + lane < D / 4) {
+        const float4 x = s_o[warp + k][c * 32 + lane];
+        sum[c].x += x.x * f, sum[c].y += x.y * f, sum[c].z += x.z * f, sum[c].w += x.w * f;
+      }
   }
+  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+  const int64_t out = static_cast<int64_t>(span.x) * p.Hq + (span.y / plan.chunks) * plan.group + chunk * 8 * NT + h;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (c * 32 + lane < D / 4)
+      reinterpret_cast<uint2*>(static_cast<act_t*>(p.out) + out * D)[c * 32 + lane] =
+          make_uint2(pack2<act_t>(sum[c].x * inv, sum[c].y * inv), pack2<act_t>(sum[c].z * inv, sum[c].w * inv));
+  if (lane == 0 && p.lse != nullptr) p.lse[out] = weight == 0.0f ? -INFINITY : (top + log2f(weight)) * LN2;
 }
 
 int tiles_of(int group) { return group <= 8 ? 1 : 2; }     // n-tiles of eight heads that a warp keeps at once
@@ -561,7 +666,7 @@ int full_grid_of(int D) {
 }
 
 int64_t workspace_bytes(int grid, int NT, int D) {
-  return static_cast<int64_t>(grid) * sizeof(int4) + static_cast<int64_t>(2 * grid) * 8 * NT * (D + 2) * 4;
+  return static_cast<int64_t>(2 * grid) * sizeof(int4) + static_cast<int64_t>(2 * grid) * 8 * NT * (D + 2) * 4;
 }
 
 // Tensor map of one cache: [page][token][head][channel], boxes of TILE tokens and 64 channels of one head. Axes of one entry get
@@ -609,6 +714,7 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
     once.mark(dev);
   }
   Plan plan;
+  plan.page = Divisor(static_cast<uint32_t>(a.block_size));
   plan.group = a.Hq / a.Hk;
   plan.chunks = (plan.group + 8 * NT - 1) / (8 * NT);
   // No more units than this, and one per (request, item) when no table row holds more than 64 tokens.
@@ -616,8 +722,8 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   const int64_t per_item = (static_cast<int64_t>(a.columns) * a.block_size + UNIT - 1) / UNIT;
   const int64_t units = per_item > (INT64_MAX / items) ? INT64_MAX : items * per_item;
   plan.grid = static_cast<int>(units < 1 ? 1 : units < full_grid<D>() ? units : full_grid<D>());
-  plan.head_part = static_cast<int4*>(a.workspace);
-  plan.part_o = reinterpret_cast<float*>(plan.head_part + plan.grid);
+  plan.spans = static_cast<int4*>(a.workspace);
+  plan.part_o = reinterpret_cast<float*>(plan.spans + 2 * plan.grid);
   plan.part_m = plan.part_o + static_cast<int64_t>(2 * plan.grid) * 8 * NT * D;
   plan.part_l = plan.part_m + static_cast<int64_t>(2 * plan.grid) * 8 * NT;
   PLA_REQUIRE(a.workspace_bytes >= workspace_bytes(plan.grid, NT, D), PLA_B200_E_INVALID, "the workspace is too small");
@@ -627,12 +733,12 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
     if (rc == PLA_B200_OK) rc = cache_map(&v_map, a, const_cast<void*>(a.v_cache), a.v_strides);
     if (rc != PLA_B200_OK) return rc;
   }
-  paged_decode_kernel<act_t, D, NT, BOXED><<<plan.grid, THREADS, S::SMEM, stream>>>(a, plan, k_map, v_map);
+  paged_decode_kernel<act_t, D, NT, BOXED><<<plan.grid, THREADS + 32, S::SMEM, stream>>>(a, plan, k_map, v_map);
   PLA_CUDA_OK(cudaGetLastError());
   if (per_item > 1) {                               // else every item is one unit and was stored whole
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(plan.grid, plan.group < 8 * NT ? plan.group : 8 * NT);
-    cfg.blockDim = dim3(THREADS);
+    cfg.gridDim = dim3(2 * plan.grid);
+    cfg.blockDim = dim3(JOIN_WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
