@@ -174,6 +174,19 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+// Division of numbers below 2^31 by a fixed d: (t * m) >> (31 + L) with L = ceil(log2 d), m = floor(2^(31 + L) / d) + 1, exact because
+// m d exceeds 2^(31 + L) by at most d <= 2^L.
+struct Divisor {
+  uint32_t d, m, shift;
+  explicit Divisor(uint32_t by = 1) : d(by), shift(31) {
+    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
+    m = static_cast<uint32_t>((uint64_t{1} << shift) / d + 1);
+  }
+  __device__ __forceinline__ int quotient(int t) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * m) >> shift);
+  }
+};
+
 // 4 consecutive 16-bit activations -> float4 (8-byte load; caller guarantees alignment).
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p) {

@@ -51,19 +51,6 @@ struct Shape {
   static constexpr int SMEM = 1024 + STAGES * STAGE + JOIN;   // the ring begins at a multiple of 1,024 bytes
 };
 
-// Division of numbers below 2^31 by a fixed d: (t * m) >> (31 + L) with L = ceil(log2 d), m = floor(2^(31 + L) / d) + 1, exact because
-// m d exceeds 2^(31 + L) by at most d <= 2^L.
-struct Divisor {
-  uint32_t d, m, shift;
-  explicit Divisor(uint32_t by = 1) : d(by), shift(31) {
-    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
-    m = static_cast<uint32_t>((uint64_t{1} << shift) / d + 1);
-  }
-  __device__ __forceinline__ int quotient(int t) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * m) >> shift);
-  }
-};
-
 struct Plan {              // of one call, the same on host and device
   Divisor page;            // by block_size
   int chunks;              // groups of 8 * NT query heads per key/value head
