@@ -5,7 +5,7 @@
 // (heads) of one token, or a share of them when there are few tokens; a row belongs to a group of 4, 8 or 16 lanes, and a lane holds
 // eight channels of the row's first half and eight of its second. With y = inv x w (inv from the group's sum of squares) and the
 // pair's other channel x', the rotated channel is inv (x A + x' B), A = w cos and B = -+ w' sin: weights, sines and cosines are folded
-// once per token and side, and a channel costs two multiply-adds, two channels to an instruction. x' is the lane's other half
+// once per token and side, and a channel costs two multiply-adds. x' is the lane's other half
 // (whole head rotated), the same lane's neighbour (interleaved), comes from the lane R/16 away as the raw 16-bit row (up to half the
 // head rotated), or from memory again where the rotated part does not fit these. Angles: the warp's lanes reduce position * frequency
 // to a fraction of a turn in 64 bits (in 32 bits whole radians are lost at positions of a million), take sine and cosine in 32 bits and
@@ -23,26 +23,33 @@ constexpr int MAX_D = 256;
 constexpr int RING = 4;          // steps in flight per warp, 1 KB each
 constexpr int BLOCKS = 2;        // CTAs per SM
 
-// Where the other channel of a pair is: HALF_LOW: R a multiple of 16, at most D / 2; HALF_FULL: R = D, a multiple of 16.
-enum Layout { HALF_LOW = 0, HALF_FULL = 1, HALF_ANY = 2, PAIRS = 3 };
+// Where the other channel of a pair is. HALF_LOW: half layout, R a multiple of 16, at most D / 2. HALF_FULL: half layout, R = D, a multiple
+// of 16. HALF_QUADS: half layout, R another multiple of 8. PAIRS: interleaved, R a multiple of 8. ANY: everything else.
+enum Layout { HALF_LOW = 0, HALF_FULL = 1, HALF_QUADS = 2, PAIRS = 3, ANY = 4 };
+
+// Queries, keys, values of one call: strides in elements, below 2^31.
+struct Side {
+  const void* in;
+  void* out;               // values: none
+  const void* weight;
+  int in_tok, in_head, out_tok, out_head, heads, first, weight_dtype;     // first: of the steps in front of this side's
+};
+struct Work {
+  Side side[3];
+  pla_b200_index positions, slots;
+  const double* inv_freq;
+  void* cache[3];          // by side; none for queries
+  pla_b200_page_strides cache_strides[3];
+  int64_t num_blocks;
+  Divisor page;
+  int T, D, R, steps, interleaved, unit_offset;
+  uint32_t split, workers;
+  float factor, eps;
+  int32_t* status;
+};
 
 __device__ __forceinline__ int64_t index_at(const pla_b200_index& x, int64_t i) {
   return x.wide ? static_cast<const int64_t*>(x.data)[i * x.stride] : static_cast<const int32_t*>(x.data)[i * x.stride];
-}
-
-// Two 32-bit numbers per instruction (the pair is one 64-bit register).
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(r))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return r;
 }
 
 template <typename act_t>
@@ -55,29 +62,40 @@ template <>
 __device__ __forceinline__ float2 widen<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+template <typename act_t>
+__device__ __forceinline__ void unpack(const uint4& raw, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 two = widen<act_t>((&raw.x)[i]);
+    x[2 * i] = two.x, x[2 * i + 1] = two.y;
+  }
+}
 
 template <typename act_t>
-__device__ __forceinline__ uint32_t narrow(float2 x);
+__device__ __forceinline__ uint32_t narrow(float lo, float hi);
 template <>
-__device__ __forceinline__ uint32_t narrow<__nv_bfloat16>(float2 x) {
+__device__ __forceinline__ uint32_t narrow<__nv_bfloat16>(float lo, float hi) {
   uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 template <>
-__device__ __forceinline__ uint32_t narrow<__half>(float2 x) {
+__device__ __forceinline__ uint32_t narrow<__half>(float lo, float hi) {
   uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+template <typename act_t>
+__device__ __forceinline__ uint4 pack(const float* x) {
+  return make_uint4(narrow<act_t>(x[0], x[1]), narrow<act_t>(x[2], x[3]), narrow<act_t>(x[4], x[5]), narrow<act_t>(x[6], x[7]));
 }
 
 // Eight numbers of shared memory.
-__device__ __forceinline__ void read8(float2* to, const float* from) {
+__device__ __forceinline__ void read8(float* to, const float* from) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float4 x = reinterpret_cast<const float4*>(from)[i];
-    to[2 * i] = make_float2(x.x, x.y);
-    to[2 * i + 1] = make_float2(x.z, x.w);
+    to[4 * i] = x.x, to[4 * i + 1] = x.y, to[4 * i + 2] = x.z, to[4 * i + 3] = x.w;
   }
 }
 
@@ -91,58 +109,64 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ float rsqrt_fast(float x) {     // relative error within 2^-22
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename act_t, int GROUP, int LAYOUT>
-__global__ void __launch_bounds__(WARPS * 32, BLOCKS)
-rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t workers, const Divisor page) {
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS) rotary_kernel(const __grid_constant__ Work p) {
   constexpr int ROWS = 32 / GROUP;                     // rows per step of a warp
   __shared__ __align__(16) uint4 s_ring[WARPS][RING][2][32];
   __shared__ __align__(16) float s_w[2][MAX_D];
   __shared__ __align__(16) float s_cos[WARPS][MAX_D / 2], s_sin[WARPS][MAX_D / 2];
-  __shared__ double s_turn[MAX_D / 2];                 // frequencies in turns per position
+  __shared__ int64_t s_turn[MAX_D / 2];                // frequencies in turns per position, units of 2^-64
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int D = p.D, R = p.R, half = R / 2;
-  const bool weights = p.q_weight != nullptr || p.k_weight != nullptr;
+  const int R = p.R, half = R / 2;
 
-  // ---- this warp: steps [begin, end) of ROWS rows each (queries, keys, values) of every token of its share
-  const uint32_t share = blockIdx.x * WARPS + warp, part = share % split;
-  const int64_t stride_t = workers / split;
-  int64_t t = share / split;
-  const int64_t tokens = share < workers ? p.T : 0;
-  const int own = lane % GROUP, sub = lane / GROUP, upper = (D + 15) / 16 * 8;
+  // ---- this warp: steps [begin, end) of ROWS rows each (queries, keys, values) of every stride_t-th token
+  const uint32_t share = blockIdx.x * WARPS + warp, part = share % p.split;
+  const int stride_t = static_cast<int>(p.workers / p.split), tokens = share < p.workers ? p.T : 0;
+  int t = static_cast<int>(share / p.split);
+  const int own = lane % GROUP, sub = lane / GROUP, upper = (p.D + 15) / 16 * 8;
   const int e[2] = {own * 8, upper + own * 8};         // the lane's channels: [e[0], e[0] + 8) and [e[1], e[1] + 8)
-  const bool on[2] = {e[0] < upper, e[0] < upper && e[1] < D};
-  const int steps_q = (p.Hq + ROWS - 1) / ROWS, steps_k = (p.Hk + ROWS - 1) / ROWS;
-  const int steps = steps_q + steps_k + (p.k_cache != nullptr ? steps_k : 0);
-  const int begin = static_cast<int>(part * static_cast<uint32_t>(steps) / split), end = static_cast<int>((part + 1) * static_cast<uint32_t>(steps) / split);
+  const bool on[2] = {e[0] < upper, e[0] < upper && e[1] < p.D};
+  const int begin = static_cast<int>(part * static_cast<uint32_t>(p.steps) / p.split);
+  const int end = static_cast<int>((part + 1) * static_cast<uint32_t>(p.steps) / p.split);
+  auto wide = [](int a, int b) { return static_cast<int64_t>(a) * b; };
 
   // ---- loads, RING steps ahead
   const uint32_t cells = smem_addr(&s_ring[warp][0][0][lane]);
-  int64_t load_t = t;
-  int load_s = begin, load_stop = 0, load_h = 0, load_heads = 0;       // the step that comes next, the end of its side, its row
+  int load_t = t, load_s = begin, load_side = begin < p.side[1].first ? 0 : begin < p.side[2].first ? 1 : 2;
+  int load_stop = 0, load_h = 0, load_heads = 0;                       // end of the side, row, rows of the side
+  int64_t load_step = 0;
   const act_t* load_ptr = nullptr;
-  int64_t load_stride = 0;
   auto enter_side = [&] {
-    const int kind = load_s < steps_q ? 0 : load_s < steps_q + steps_k ? 1 : 2;
-    const int start = kind == 0 ? 0 : kind == 1 ? steps_q : steps_q + steps_k;
-    load_h = (load_s - start) * ROWS + sub;
-    load_heads = kind == 0 ? p.Hq : p.Hk;
-    load_stop = min(end, start + (kind == 0 ? steps_q : steps_k));
-    const int64_t head = kind == 0 ? p.q_head_stride : kind == 1 ? p.k_head_stride : p.v_head_stride;
-    const int64_t tok = kind == 0 ? p.q_tok_stride : kind == 1 ? p.k_tok_stride : p.v_tok_stride;
-    load_ptr = static_cast<const act_t*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + load_t * tok + load_h * head + e[0];
-    load_stride = ROWS * head;
+    const Side& x = p.side[load_side];
+    load_h = (load_s - x.first) * ROWS + sub;
+    load_heads = x.heads;
+    load_stop = load_side == 2 ? end : min(end, p.side[load_side + 1].first);
+    load_step = wide(ROWS, x.in_head);
+    load_ptr = static_cast<const act_t*>(x.in) + e[0] + wide(load_t, x.in_tok) + wide(load_h, x.in_head);
   };
-  auto issue = [&](int slot) {
+  auto issue = [&](int cell) {
     if (load_t < tokens) {
-      const uint32_t to = cells + slot * 1024;
+      const uint32_t to = cells + cell * 1024;
       if (load_h < load_heads) {
         if (on[0]) copy16(to, load_ptr);
         if (on[1]) copy16(to + 512, load_ptr + upper);
       }
       load_h += ROWS;
-      load_ptr += load_stride;
+      load_ptr += load_step;
       if (++load_s == load_stop) {
-        if (load_s == end) load_s = begin, load_t += stride_t;
+        if (load_s == end) {
+          load_s = begin;
+          load_t = load_t < tokens - stride_t ? load_t + stride_t : tokens;
+          load_side = begin < p.side[1].first ? 0 : begin < p.side[2].first ? 1 : 2;
+        } else {
+          do ++load_side; while (load_side < 2 && p.side[load_side + 1].first <= load_s);
+        }
         enter_side();                                  // past the last token: an address that is not used
       }
     }
@@ -151,19 +175,21 @@ rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t
 #pragma unroll
   for (int i = 0; i < RING; ++i) s_ring[warp][i][0][lane] = s_ring[warp][i][1][lane] = make_uint4(0, 0, 0, 0);   // channels past D stay 0
   enter_side();
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < RING; ++i) issue(i);
 
   // ---- what all tokens share
-  for (int i = tid; i < half; i += WARPS * 32) s_turn[i] = p.inv_freq[i] * 0.15915494309189535;   // 1 / (2 pi)
-  if (weights) {
-    for (int i = tid; i < 2 * D; i += WARPS * 32) {
-      const int side = i >= D;
-      const void* w = side ? p.k_weight : p.q_weight;
-      s_w[side][i - side * D] = w == nullptr ? 1.0f : load_any(w, side ? p.k_weight_dtype : p.q_weight_dtype, i - side * D) + (p.unit_offset ? 1.0f : 0.0f);
-    }
+  for (int i = tid; i < half; i += WARPS * 32) {
+    const double turns = p.inv_freq[i] * 0.15915494309189535;          // 1 / (2 pi)
+    s_turn[i] = __double2ll_rn((turns - rint(turns)) * 18446744073709551616.0);
   }
-  const bool turns_any = begin < steps_q + steps_k, caches = p.k_cache != nullptr && end > steps_q;
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const void* w = p.side[side].weight;
+    if (w != nullptr)
+      for (int i = tid; i < p.D; i += WARPS * 32) s_w[side][i] = load_any(w, p.side[side].weight_dtype, i) + (p.unit_offset ? 1.0f : 0.0f);
+  }
+  const bool turns_any = begin < p.side[2].first, caches = p.cache[1] != nullptr && end > p.side[1].first;
   int64_t position = 0, slot = -1;
   if (t < tokens) {
     if (turns_any) position = index_at(p.positions, t);
@@ -171,80 +197,119 @@ rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t
   }
   const int r16 = R / 16;
   const int mate_lane = own < r16 ? lane + r16 : own < 2 * r16 ? lane - r16 : lane;
-  const float inv_d = 1.0f / static_cast<float>(D);
+  const float inv_d = 1.0f / static_cast<float>(p.D);
   float* const cosines = s_cos[warp];
   float* const sines = s_sin[warp];
-  int ring = 0;
+  int cell = 0;
   __syncthreads();
 
 #pragma unroll 1
-  for (; t < tokens; t += stride_t) {
+  for (; t < tokens; t = t < tokens - stride_t ? t + stride_t : tokens) {
     if (turns_any) {
+#pragma unroll 1
       for (int i = lane; i < half; i += 32) {
-        const double turns = static_cast<double>(position) * s_turn[i];
-        const float frac = static_cast<float>(turns - rint(turns));
+        // the product wraps at whole turns; its upper half is the fraction in units of 2^-32
+        const int frac = static_cast<int>(static_cast<uint64_t>(position) * static_cast<uint64_t>(s_turn[i]) >> 32);
         float sn, cs;
-        sincospif(2.0f * frac, &sn, &cs);
+        sincospif(static_cast<float>(frac) * 4.656612873077393e-10f, &sn, &cs);      // 2^-31: half turns
         cosines[i] = cs * p.factor;
         sines[i] = sn * p.factor;
       }
     }
-    int64_t k_at = -1, v_at = -1;          // where the token's rows go in the caches
+    int64_t block = -1, off = 0;           // where the token's rows go in the caches
     if (slot >= 0) {
-      const int64_t block = slot <= INT32_MAX ? page.quotient(static_cast<int>(slot)) : slot / p.block_size, off = slot - block * p.block_size;
-      if (block < p.num_blocks) {
-        k_at = block * p.k_strides.block + off * p.k_strides.token;
-        v_at = block * p.v_strides.block + off * p.v_strides.token;
-      } else if (lane == 0 && p.status != nullptr) {
-        atomicOr(p.status, PLA_B200_DEV_BAD_SLOT);
+      block = slot <= INT32_MAX ? p.page.quotient(static_cast<int>(slot)) : slot / p.page.d;
+      off = slot - block * p.page.d;
+      if (block >= p.num_blocks) {
+        block = -1;
+        if (lane == 0 && p.status != nullptr) atomicOr(p.status, PLA_B200_DEV_BAD_SLOT);
       }
     }
-    if (t + stride_t < tokens) {           // of the next token
+    if (t < tokens - stride_t) {           // of the next token
       if (turns_any) position = index_at(p.positions, t + stride_t);
       if (caches) slot = index_at(p.slots, t + stride_t);
     }
     __syncwarp();
 
 #pragma unroll 1
-    for (int side = 0; side < 2; ++side) {
-      const int first = side == 0 ? begin : max(begin, steps_q), last = side == 0 ? min(end, steps_q) : min(end, steps_q + steps_k);
+    for (int side = 0; side < 3; ++side) {
+      const Side& z = p.side[side];
+      const int first = max(begin, z.first), last = side == 2 ? end : min(end, p.side[side + 1].first);
       if (first >= last) continue;
-      const bool normed = (side == 0 ? p.q_weight : p.k_weight) != nullptr, stored = side == 1 && k_at >= 0;
-      const int heads = side == 0 ? p.Hq : p.Hk;
-      int h = (first - (side == 0 ? 0 : steps_q)) * ROWS + sub;
-      const int64_t out_step = ROWS * (side == 0 ? p.qo_head_stride : p.ko_head_stride), cache_step = ROWS * p.k_strides.head;
-      act_t* out = static_cast<act_t*>(side == 0 ? p.q_out : p.k_out);
-      const bool dense = out != nullptr;
-      out += t * (side == 0 ? p.qo_tok_stride : p.ko_tok_stride) + h * (side == 0 ? p.qo_head_stride : p.ko_head_stride) + e[0];
-      act_t* cached = static_cast<act_t*>(p.k_cache) + k_at + h * p.k_strides.head + e[0];
+      const int heads = z.heads;
+      int h = (first - z.first) * ROWS + sub;
+      act_t* cached = nullptr;
+      const int64_t cache_step = ROWS * p.cache_strides[side].head;
+      if (side > 0 && block >= 0)
+        cached = static_cast<act_t*>(p.cache[side]) + block * p.cache_strides[side].block + off * p.cache_strides[side].token +
+                 h * p.cache_strides[side].head + e[0];
+      if (side == 2) {                     // values: copied
+#pragma unroll 1
+        for (int s = first; s < last; ++s) {
+          wait_copies<RING - 1>();
+          if (cached != nullptr) {
+            if (h < heads) {
+              if (on[0]) *reinterpret_cast<uint4*>(cached) = s_ring[warp][cell][0][lane];
+              if (on[1]) *reinterpret_cast<uint4*>(cached + upper) = s_ring[warp][cell][1][lane];
+            }
+            cached += cache_step;
+          }
+          issue(cell);
+          cell = cell + 1 == RING ? 0 : cell + 1;
+          h += ROWS;
+        }
+        break;
+      }
+      const bool normed = z.weight != nullptr, dense = z.out != nullptr;
+      act_t* out = static_cast<act_t*>(z.out) + e[0] + wide(t, z.out_tok) + wide(h, z.out_head);
+      const int64_t out_step = wide(ROWS, z.out_head);
 
       // weights, sines and cosines of the lane's channels
-      float2 A[2][4], B[2][4];
+      float A[2][8], B[2][8];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) A[c][i] = make_float2(1.0f, 1.0f), B[c][i] = make_float2(0.0f, 0.0f);
+        for (int i = 0; i < 8; ++i) A[c][i] = 1.0f, B[c][i] = 0.0f;
         if (LAYOUT == HALF_LOW && c == 1) continue;
-        if (LAYOUT == HALF_LOW || LAYOUT == HALF_FULL) {
-          if (e[c] < R && on[c]) {
+        if (LAYOUT == ANY) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = e[c] + i;
+            if (at < R && on[c]) {
+              const bool second = p.interleaved ? (i & 1) : at >= half;
+              const int f = p.interleaved ? at >> 1 : second ? at - half : at;
+              A[c][i] = cosines[f];
+              B[c][i] = second ? sines[f] : -sines[f];
+            }
+          }
+        } else if (LAYOUT == HALF_QUADS) {     // four channels at a time: half is a multiple of four
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const int at = e[c] + i;
+            if (at < R && on[c]) {
+              const bool second = at >= half;
+              const int f = second ? at - half : at;
+              const float4 cs = *reinterpret_cast<const float4*>(cosines + f), sn = *reinterpret_cast<const float4*>(sines + f);
+              const float sign = second ? 1.0f : -1.0f;
+              A[c][i] = cs.x, A[c][i + 1] = cs.y, A[c][i + 2] = cs.z, A[c][i + 3] = cs.w;
+              B[c][i] = sign * sn.x, B[c][i + 1] = sign * sn.y, B[c][i + 2] = sign * sn.z, B[c][i + 3] = sign * sn.w;
+            }
+          }
+        } else if (e[c] < R && on[c]) {
+          if (LAYOUT == PAIRS) {
+            const float4 cs = *reinterpret_cast<const float4*>(cosines + e[c] / 2), sn = *reinterpret_cast<const float4*>(sines + e[c] / 2);
+            A[c][0] = A[c][1] = cs.x, A[c][2] = A[c][3] = cs.y, A[c][4] = A[c][5] = cs.z, A[c][6] = A[c][7] = cs.w;
+            B[c][1] = sn.x, B[c][3] = sn.y, B[c][5] = sn.z, B[c][7] = sn.w;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) B[c][i] = -B[c][i + 1];
+          } else {
             const bool second = e[c] >= half;
             const int f = second ? e[c] - half : e[c];
             const float sign = second ? 1.0f : -1.0f;
             read8(A[c], cosines + f);
             read8(B[c], sines + f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) B[c][i] = mul2(B[c][i], make_float2(sign, sign));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = e[c] + i;
-            if (at < R && on[c]) {
-              const bool second = LAYOUT == PAIRS ? (i & 1) : at >= half;
-              const int f = LAYOUT == PAIRS ? at >> 1 : second ? at - half : at;
-              reinterpret_cast<float*>(A[c])[i] = cosines[f];
-              reinterpret_cast<float*>(B[c])[i] = second ? sines[f] : -sines[f];
-            }
+            for (int i = 0; i < 8; ++i) B[c][i] *= sign;
           }
         }
       }
@@ -252,24 +317,33 @@ rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (!on[c]) continue;
-          float2 w[4];
+          float w[8];
           read8(w, s_w[side] + e[c]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) A[c][i] = mul2(A[c][i], w[i]);
+          for (int i = 0; i < 8; ++i) A[c][i] *= w[i];
           if (LAYOUT == HALF_LOW && c == 1) continue;
           if (LAYOUT == PAIRS) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) B[c][i] = mul2(B[c][i], make_float2(w[i].y, w[i].x));
-          } else if (LAYOUT == HALF_ANY) {
+            for (int i = 0; i < 8; ++i) B[c][i] *= w[i ^ 1];
+          } else if (LAYOUT == ANY) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int at = e[c] + i;
-              if (at < R) reinterpret_cast<float*>(B[c])[i] *= s_w[side][at < half ? at + half : at - half];
+              if (at < R) B[c][i] *= s_w[side][p.interleaved ? at ^ 1 : at < half ? at + half : at - half];
+            }
+          } else if (LAYOUT == HALF_QUADS) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const int at = e[c] + i;
+              if (at < R) {
+                const float4 m = *reinterpret_cast<const float4*>(s_w[side] + (at < half ? at + half : at - half));
+                B[c][i] *= m.x, B[c][i + 1] *= m.y, B[c][i + 2] *= m.z, B[c][i + 3] *= m.w;
+              }
             }
           } else if (e[c] < R) {
             read8(w, s_w[side] + (e[c] < half ? e[c] + half : e[c] - half));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) B[c][i] = mul2(B[c][i], w[i]);
+            for (int i = 0; i < 8; ++i) B[c][i] *= w[i];
           }
         }
       }
@@ -277,81 +351,91 @@ rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t
 #pragma unroll 1
       for (int s = first; s < last; ++s) {
         wait_copies<RING - 1>();
-        if (LAYOUT == HALF_ANY) __syncwarp();
-        const uint4 raw[2] = {s_ring[warp][ring][0][lane], s_ring[warp][ring][1][lane]};
-        float2 x[2][4], y[2][4];
+        if (LAYOUT == ANY || LAYOUT == HALF_QUADS) __syncwarp();     // the mate's cell may be another lane's copy
+        const uint4 raw[2] = {s_ring[warp][cell][0][lane], s_ring[warp][cell][1][lane]};
+        float x[2][8], y[2][8];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
+          unpack<act_t>(raw[c], x[c]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[c][i] = widen<act_t>((&raw[c].x)[i]), y[c][i] = mul2(x[c][i], A[c][i]);
+          for (int i = 0; i < 8; ++i) y[c][i] = x[c][i] * A[c][i];
+        }
+        // the pairs' other channels; channels past R are left out, 0 * infinity must not enter
         if constexpr (LAYOUT == HALF_LOW) {
+          uint4 other;
+          other.x = __shfl_sync(0xffffffffu, raw[0].x, mate_lane);
+          other.y = __shfl_sync(0xffffffffu, raw[0].y, mate_lane);
+          other.z = __shfl_sync(0xffffffffu, raw[0].z, mate_lane);
+          other.w = __shfl_sync(0xffffffffu, raw[0].w, mate_lane);
+          if (e[0] < R) {
+            float z[8];
+            unpack<act_t>(other, z);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t other = __shfl_sync(0xffffffffu, (&raw[0].x)[i], mate_lane);
-            y[0][i] = fma2(widen<act_t>(e[0] < R ? other : 0), B[0][i], y[0][i]);     // copied channels: 0 * infinity must not enter
+            for (int i = 0; i < 8; ++i) y[0][i] = fmaf(z[i], B[0][i], y[0][i]);
           }
         } else if constexpr (LAYOUT == HALF_FULL) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[0][i] = fma2(x[1][i], B[0][i], y[0][i]), y[1][i] = fma2(x[0][i], B[1][i], y[1][i]);
+          for (int i = 0; i < 8; ++i) y[0][i] = fmaf(x[1][i], B[0][i], y[0][i]), y[1][i] = fmaf(x[0][i], B[1][i], y[1][i]);
         } else if constexpr (LAYOUT == PAIRS) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
+            if (e[c] < R) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              y[c][i] = fma2(e[c] + 2 * i < R ? make_float2(x[c][i].y, x[c][i].x) : make_float2(0.0f, 0.0f), B[c][i], y[c][i]);
+              for (int i = 0; i < 8; ++i) y[c][i] = fmaf(x[c][i ^ 1], B[c][i], y[c][i]);
+            }
+        } else if constexpr (LAYOUT == HALF_QUADS) {
+          const act_t* pieces = reinterpret_cast<const act_t*>(&s_ring[warp][cell][0][sub * GROUP]);    // the row's, 256 channels apart
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const int at = e[c] + i, mate = at < half ? at + half : at - half;
+              if (on[c] && at < R) {
+                const uint2 four = *reinterpret_cast<const uint2*>(pieces + (mate < upper ? mate : mate - upper + 256));
+                const float2 lo = widen<act_t>(four.x), hi = widen<act_t>(four.y);
+                y[c][i] = fmaf(lo.x, B[c][i], y[c][i]);
+                y[c][i + 1] = fmaf(lo.y, B[c][i + 1], y[c][i + 1]);
+                y[c][i + 2] = fmaf(hi.x, B[c][i + 2], y[c][i + 2]);
+                y[c][i + 3] = fmaf(hi.y, B[c][i + 3], y[c][i + 3]);
+              }
+            }
+          __syncwarp();                                       // the cells are filled again
         } else {
-          const act_t* pieces = reinterpret_cast<const act_t*>(&s_ring[warp][ring][0][sub * GROUP]);    // the row's, 256 channels apart
+          const act_t* pieces = reinterpret_cast<const act_t*>(&s_ring[warp][cell][0][sub * GROUP]);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int at = e[c] + i, mate = at < half ? at + half : at - half;
-              const float other = on[c] && at < R ? to_f32(pieces[mate < upper ? mate : mate - upper + 256]) : 0.0f;
-              reinterpret_cast<float*>(y[c])[i] = fmaf(other, reinterpret_cast<float*>(B[c])[i], reinterpret_cast<float*>(y[c])[i]);
+              const int at = e[c] + i, mate = p.interleaved ? at ^ 1 : at < half ? at + half : at - half;
+              if (on[c] && at < R) y[c][i] = fmaf(to_f32(pieces[mate < upper ? mate : mate - upper + 256]), B[c][i], y[c][i]);
             }
           __syncwarp();                                       // the cells are filled again
         }
         if (normed) {
-          float2 q2 = mul2(x[0][0], x[0][0]);
+          float sq = 0.0f;
 #pragma unroll
-          for (int i = 1; i < 8; ++i) q2 = fma2(x[i / 4][i % 4], x[i / 4][i % 4], q2);
-          float sq = q2.x + q2.y;
+          for (int i = 0; i < 16; ++i) sq = fmaf(x[i / 8][i % 8], x[i / 8][i % 8], sq);
 #pragma unroll
           for (int o = GROUP / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float inv = rsqrtf(fmaf(sq, inv_d, p.eps));
+          const float inv = rsqrt_fast(fmaf(sq, inv_d, p.eps));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i / 4][i % 4] = mul2(y[i / 4][i % 4], make_float2(inv, inv));
+          for (int i = 0; i < 16; ++i) y[i / 8][i % 8] *= inv;
         }
         if (h < heads) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (!on[c]) continue;
-            const uint4 packed = make_uint4(narrow<act_t>(y[c][0]), narrow<act_t>(y[c][1]), narrow<act_t>(y[c][2]), narrow<act_t>(y[c][3]));
+            const uint4 packed = pack<act_t>(y[c]);
             if (dense) *reinterpret_cast<uint4*>(out + c * upper) = packed;
-            if (stored) *reinterpret_cast<uint4*>(cached + c * upper) = packed;
+            if (cached != nullptr) *reinterpret_cast<uint4*>(cached + c * upper) = packed;
           }
         }
-        issue(ring);
-        ring = ring + 1 == RING ? 0 : ring + 1;
+        issue(cell);
+        cell = cell + 1 == RING ? 0 : cell + 1;
         h += ROWS;
         out += out_step;
-        cached += cache_step;
+        if (cached != nullptr) cached += cache_step;
       }
-    }
-
-    // values: copied
-#pragma unroll 1
-    for (int s = max(begin, steps_q + steps_k); s < end; ++s) {
-      wait_copies<RING - 1>();
-      const int h = (s - steps_q - steps_k) * ROWS + sub;
-      if (h < p.Hk && v_at >= 0) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (on[c])
-            *reinterpret_cast<uint4*>(static_cast<act_t*>(p.v_cache) + v_at + h * p.v_strides.head + e[c]) = s_ring[warp][ring][c][lane];
-      }
-      issue(ring);
-      ring = ring + 1 == RING ? 0 : ring + 1;
     }
     __syncwarp();                          // the next token overwrites sines and cosines
   }
@@ -361,19 +445,40 @@ rotary_kernel(const pla_b200_rotary_args p, const uint32_t split, const uint32_t
 template <typename act_t, int GROUP>
 int launch(const pla_b200_rotary_args& a, cudaStream_t stream) {
   constexpr int ROWS = 32 / GROUP;
-  const int64_t steps = (a.Hq + ROWS - 1) / ROWS + static_cast<int64_t>((a.Hk + ROWS - 1) / ROWS) * (a.k_cache != nullptr ? 2 : 1);
+  const bool cached = a.k_cache != nullptr;
+  const int steps_q = (a.Hq + ROWS - 1) / ROWS, steps_k = (a.Hk + ROWS - 1) / ROWS;
+  auto i = [](int64_t x) { return static_cast<int>(x); };
+  Work w = {};
+  w.side[0] = {a.q, a.q_out, a.q_weight, i(a.q_tok_stride), i(a.q_head_stride), i(a.qo_tok_stride), i(a.qo_head_stride), a.Hq, 0, a.q_weight_dtype};
+  w.side[1] = {a.k, a.k_out, a.k_weight, i(a.k_tok_stride), i(a.k_head_stride), i(a.ko_tok_stride), i(a.ko_head_stride), a.Hk, steps_q, a.k_weight_dtype};
+  w.side[2] = {a.v, nullptr, nullptr, i(a.v_tok_stride), i(a.v_head_stride), 0, 0, cached ? a.Hk : 0, steps_q + steps_k, 0};
+  w.positions = a.positions;
+  w.inv_freq = a.inv_freq;
+  if (cached) {
+    w.slots = a.slots;
+    w.cache[1] = a.k_cache;
+    w.cache[2] = a.v_cache;
+    w.cache_strides[1] = a.k_strides;
+    w.cache_strides[2] = a.v_strides;
+    w.num_blocks = a.num_blocks;
+    w.page = Divisor(static_cast<uint32_t>(a.block_size));
+  }
+  w.T = a.T, w.D = a.D, w.R = a.R, w.interleaved = a.interleaved, w.unit_offset = a.unit_offset;
+  w.steps = steps_q + steps_k * (cached ? 2 : 1);
+  w.factor = a.factor, w.eps = a.eps, w.status = a.status;
   // A warp per token once that fills the SMs; with fewer tokens their steps are shared out.
   const int64_t full = static_cast<int64_t>(sm_count()) * BLOCKS * WARPS;
   int64_t split = full / a.T;
-  split = split < 1 ? 1 : split > steps ? steps : split;
-  int64_t workers = a.T * split < full ? a.T * split : full / split * split;
+  split = split < 1 ? 1 : split > w.steps ? w.steps : split;
+  const int64_t workers = a.T * split < full ? a.T * split : full / split * split;
+  w.split = static_cast<uint32_t>(split);
+  w.workers = static_cast<uint32_t>(workers);
   const unsigned grid = static_cast<unsigned>((workers + WARPS - 1) / WARPS);
-  const uint32_t n = static_cast<uint32_t>(split), w = static_cast<uint32_t>(workers);
-  const Divisor page(a.k_cache != nullptr ? static_cast<uint32_t>(a.block_size) : 1u);
-  if (a.interleaved) rotary_kernel<act_t, GROUP, PAIRS><<<grid, WARPS * 32, 0, stream>>>(a, n, w, page);
-  else if (a.R % 16 == 0 && 2 * a.R <= a.D) rotary_kernel<act_t, GROUP, HALF_LOW><<<grid, WARPS * 32, 0, stream>>>(a, n, w, page);
-  else if (a.R % 16 == 0 && a.R == a.D) rotary_kernel<act_t, GROUP, HALF_FULL><<<grid, WARPS * 32, 0, stream>>>(a, n, w, page);
-  else rotary_kernel<act_t, GROUP, HALF_ANY><<<grid, WARPS * 32, 0, stream>>>(a, n, w, page);
+  if (a.R % 8 != 0) rotary_kernel<act_t, GROUP, ANY><<<grid, WARPS * 32, 0, stream>>>(w);
+  else if (a.interleaved) rotary_kernel<act_t, GROUP, PAIRS><<<grid, WARPS * 32, 0, stream>>>(w);
+  else if (a.R % 16 == 0 && 2 * a.R <= a.D) rotary_kernel<act_t, GROUP, HALF_LOW><<<grid, WARPS * 32, 0, stream>>>(w);
+  else if (a.R % 16 == 0 && a.R == a.D) rotary_kernel<act_t, GROUP, HALF_FULL><<<grid, WARPS * 32, 0, stream>>>(w);
+  else rotary_kernel<act_t, GROUP, HALF_QUADS><<<grid, WARPS * 32, 0, stream>>>(w);
   PLA_CUDA_OK(cudaGetLastError());
   return PLA_B200_OK;
 }
@@ -402,6 +507,10 @@ extern "C" int pla_b200_rotary(const pla_b200_rotary_args* args, void* stream) {
                   (a.inv_freq || a.R == 0),
               PLA_B200_E_INVALID, "q, k, their outputs, positions and inv_freq are required");
   if (a.Hk == 0) a.k_cache = nullptr;
+  for (const int64_t stride : {a.q_tok_stride, a.q_head_stride, a.k_tok_stride, a.k_head_stride, a.v_tok_stride, a.v_head_stride, a.qo_tok_stride,
+                               a.qo_head_stride, a.ko_tok_stride, a.ko_head_stride})
+    PLA_REQUIRE(stride >= 0 && stride <= INT32_MAX, PLA_B200_E_TOO_LARGE, "token and head strides must be below 2^31 elements");
+  PLA_REQUIRE(a.Hq < 65536 && a.Hk < 65536, PLA_B200_E_TOO_LARGE, "too many heads");
   if (a.k_cache != nullptr) {
     PLA_REQUIRE(a.v_cache && a.v && a.slots.data && a.num_blocks >= 0 && a.block_size > 0, PLA_B200_E_INVALID,
                 "a cache needs k_cache, v_cache, v, slots, num_blocks >= 0 and block_size > 0");

@@ -238,7 +238,8 @@ def expect(x, w, pos, freq, inter, factor=1.0, unit=False, eps=1e-6):
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("T,hq,hk,D,R", [(1, 1, 1, 8, 2), (1, 32, 8, 128, 128), (3, 16, 2, 256, 64), (130, 5, 1, 96, 48), (7, 6, 3, 80, 20),
                                          (2, 40, 8, 64, 64), (17, 3, 3, 192, 192), (5, 4, 4, 256, 256), (9, 2, 1, 128, 40), (4, 3, 2, 24, 6),
-                                         (1025, 4, 2, 64, 32), (3, 2, 1, 64, 0)])
+                                         (1025, 4, 2, 64, 32), (3, 2, 1, 64, 0), (2500, 6, 2, 96, 72), (6, 9, 2, 256, 168),
+                                         (4, 3, 2, 200, 200), (3, 5, 5, 72, 40), (5001, 3, 1, 128, 128)])
 def test_rotary_matches_the_oracle(native_built, T, hq, hk, D, R, inter, dtype):
     g = torch.Generator().manual_seed(T * 7 + D + R)
     row, (q, k, _) = rows(g, T, hq, hk, D, DT[dtype], extra=8)
@@ -262,7 +263,8 @@ def test_rotary_matches_the_oracle(native_built, T, hq, hk, D, R, inter, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,wdtype", [("bf16", torch.bfloat16), ("fp16", torch.float32)])
 @pytest.mark.parametrize("inter,unit", [(False, True), (True, False)])
-@pytest.mark.parametrize("T,hq,hk,D,R", [(1, 1, 1, 8, 8), (1, 16, 2, 256, 64), (67, 5, 1, 96, 48), (6, 7, 7, 128, 128), (33, 4, 2, 64, 20), (3, 2, 1, 200, 64)])
+@pytest.mark.parametrize("T,hq,hk,D,R", [(1, 1, 1, 8, 8), (1, 16, 2, 256, 64), (67, 5, 1, 96, 48), (6, 7, 7, 128, 128), (33, 4, 2, 64, 20), (3, 2, 1, 200, 64), (2400, 3, 2, 128, 40),
+                                         (5, 2, 2, 104, 88)])
 def test_norm_rotary_matches_the_oracle(native_built, T, hq, hk, D, R, inter, unit, dtype, wdtype):
     g = torch.Generator().manual_seed(T + D + R)
     row, (q, k, _) = rows(g, T, hq, hk, D, DT[dtype])
