@@ -110,7 +110,7 @@ def build_ops(force: bool = False, verbose: bool = False) -> Path:
         objs = list(pool.map(compile_one, sources))
     torch_lib = Path(torch.__file__).parent / "lib"
     cmd = [cxx, "-shared", "-o", str(OPS_LIB), *map(str, objs),
-           f"-L{LIB}", "-lpla_b200", f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-ltorch", "-lc10_cuda",
+           f"-L{LIB}", "-lpla_b200", f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_cuda", "-lc10_cuda",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
