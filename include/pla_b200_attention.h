@@ -111,12 +111,14 @@ typedef struct pla_b200_paged_decode_args {
   int32_t B, Hq, Hk, D; /* D: 64, 96, 128, 192 or 256 */
   int32_t act_dtype;    /* BF16 or F16, of q, both caches and out */
   float scale;
-  void* workspace;      /* device scratch of pla_b200_paged_decode_workspace_bytes() bytes, 16-byte aligned; used by this call alone */
+  void* workspace;      /* device scratch of pla_b200_paged_decode_workspace_bytes() bytes, 16-byte aligned; used by this call alone,
+                           any contents. May be NULL when that is 0 */
   int64_t workspace_bytes;
   int32_t* status;
 } pla_b200_paged_decode_args;
 
-int64_t pla_b200_paged_decode_workspace_bytes(int32_t B, int32_t Hq, int32_t Hk, int32_t D);
+/* Bytes for a call with these sizes (B, Hq, Hk, D, columns, block_size are read) on the current device, or a negative code. */
+int64_t pla_b200_paged_decode_workspace_bytes(const pla_b200_paged_decode_args* args);
 int pla_b200_paged_decode(const pla_b200_paged_decode_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -99,7 +99,7 @@ def load() -> ctypes.CDLL:
     lib.pla_b200_kda_chunk_workspace_bytes.restype = ctypes.c_int64
     lib.pla_b200_kda_chunk_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32]
     lib.pla_b200_paged_decode_workspace_bytes.restype = ctypes.c_int64
-    lib.pla_b200_paged_decode_workspace_bytes.argtypes = [ctypes.c_int32] * 4
+    lib.pla_b200_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(ATTENTION_STRUCTS["pla_b200_paged_decode_args"]["class"])]
     lib.pla_b200_device_status.restype = ctypes.c_int
     lib.pla_b200_device_status.argtypes = [ctypes.POINTER(ctypes.c_int32), ctypes.c_int]
     return lib

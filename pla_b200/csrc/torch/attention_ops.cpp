@@ -291,7 +291,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_decode(const at::Tensor& q, c
                     p[b * table.size(1) + j], " of request ", b, " is outside the pool of ", c.blocks);
     }
   }
-  const int64_t bytes = pla_b200_paged_decode_workspace_bytes(g.B, g.Hq, g.Hk, g.D);
+  const int64_t bytes = pla_b200_paged_decode_workspace_bytes(&g);
+  TORCH_CHECK(bytes >= 0, "paged_attention_decode: ", pla_b200_last_error());
   at::Tensor workspace;
   if (bytes > 0) {
     workspace = fresh({bytes}, at::kByte, device);

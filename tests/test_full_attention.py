@@ -109,7 +109,13 @@ def test_abi_entries_are_exported_and_refuse_bad_arguments(native_built):
     assert lib.pla_b200_paged_decode(ctypes.byref(a), None) == -3 and b"head size" in lib.pla_b200_last_error()
     a = capi.pla_b200_paged_decode_args(B=1, Hq=4, Hk=2, D=64, block_size=4)
     assert lib.pla_b200_paged_decode(ctypes.byref(a), None) == -1 and b"required" in lib.pla_b200_last_error()
-    assert lib.pla_b200_paged_decode_workspace_bytes(-1, 4, 2, 64) == -1
+    assert lib.pla_b200_paged_decode_workspace_bytes(None) == -1
+    a = capi.pla_b200_paged_decode_args(B=64, Hq=4, Hk=3, D=64, block_size=16, columns=9)
+    assert lib.pla_b200_paged_decode_workspace_bytes(ctypes.byref(a)) == -1
+    a.Hk = 2
+    assert lib.pla_b200_paged_decode_workspace_bytes(ctypes.byref(a)) > 0
+    a.B = 1                                       # little work: clusters, no workspace
+    assert lib.pla_b200_paged_decode_workspace_bytes(ctypes.byref(a)) == 0
     r = capi.pla_b200_rotary_args(T=1, Hq=4, D=60, R=8)
     assert lib.pla_b200_rotary(ctypes.byref(r), None) == -1 and b"multiple of 8" in lib.pla_b200_last_error()
     r = capi.pla_b200_rotary_args(T=1, Hq=4, D=64, R=9)
@@ -448,6 +454,32 @@ def test_attention_lengths(native_built, lens, hq, hk, D, bs):
     q, kc, vc, table = paged_inputs(len(lens) + D, lens, hq, hk, D, bs)
     out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), return_lse=True, scale=0.11)
     assert_attention(out, lse, q, kc, vc, table, lens, 0.11)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lens,hq,hk,D,bs,layout", [([777], 16, 2, 128, 16, "separate"), ([1], 4, 4, 64, 1, "heads"), ([0, 70, 513], 8, 2, 256, 32, "packed"),
+                                                    ([4000], 5, 1, 64, 48, "separate"), ([129, 64, 0, 1], 40, 2, 96, 7, "packed"), ([300, 2000], 16, 1, 192, 64, "heads"),
+                                                    ([0], 2, 1, 128, 16, "separate"), ([600, 1023], 33, 1, 128, 8, "separate")],
+                         ids=["777", "one", "empty-first", "4000", "wide-groups", "192", "nothing", "page-8"])
+def test_attention_little_work(native_built, lens, hq, hk, D, bs, layout, dtype):
+    """Few heads and short table rows, which clusters take."""
+    from pla_b200 import capi
+    import ctypes
+    q, kc, vc, table = paged_inputs(len(lens) * D + hq, lens, hq, hk, D, bs, DT[dtype], layout, extra_columns=0)
+    a = capi.pla_b200_paged_decode_args(B=len(lens), Hq=hq, Hk=hk, D=D, block_size=bs, columns=table.shape[1])
+    assert capi.load().pla_b200_paged_decode_workspace_bytes(ctypes.byref(a)) == 0
+    status = word()
+    out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), return_lse=True, status=status)
+    assert status.item() == 0
+    assert_attention(out, lse, q, kc, vc, table, lens)
+    again = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), out=torch.full_like(out, float("nan")))
+    assert torch.equal(again, out)
+    # a wide table takes the other way: the same values within both ways' bounds
+    wide = torch.full((len(lens), 20000 // bs + 1), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, wide.cuda(), i32(lens), return_lse=True)
+    assert_attention(out, lse, q, kc, vc, table, lens)
 
 
 @pytest.mark.gpu
