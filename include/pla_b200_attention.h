@@ -32,7 +32,8 @@ typedef struct pla_b200_page_strides {
  * block_table[n, p / block_size] * block_size + p % block_size. Other entries of the table keep their values. Tokens at or past
  * query_start_loc[N], tokens without a page and tokens of a request with bad metadata (c < 0, m < 0 or c + m past 32 bits:
  * it takes no pages, seq_lens[n] = max(c, 0), PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last
- * kind. A page past the end of the free list becomes -1. Outputs must not overlap inputs (block_table is both).
+ * kind. A page past the end of the free list becomes -1. `tokens` has to cover query_start_loc[N]; where it does not, the rest is
+ * left out (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs (block_table is both).
  * ======================================================================== */
 typedef struct pla_b200_block_tables_args {
   int32_t* block_table;           /* [N, columns], pages of the context already in place */
@@ -93,7 +94,7 @@ int pla_b200_rotary(const pla_b200_rotary_args* args, void* stream);
  *   s_j = scale * q . k_j,  j < seq_lens[b];  lse = log(sum exp(s_j));  out = sum exp(s_j - lse) v_j
  * Query head h reads key/value head h / (Hq / Hk). A request of length 0 gets zeros and lse = -inf. Token j sits in page
  * block_table[b, j / block_size]; nothing at or past seq_lens[b] is read. A length < 0 (taken as 0) or past the table's
- * columns (cut there) sets PLA_B200_DEV_BAD_INTERVAL; tokens whose page lies outside the pool are left out and set PLA_B200_DEV_BAD_SLOT.
+ * columns or 2^30 (cut there) sets PLA_B200_DEV_BAD_INTERVAL; tokens whose page lies outside the pool are left out and set PLA_B200_DEV_BAD_SLOT.
  * ======================================================================== */
 typedef struct pla_b200_paged_decode_args {
   const void* q;        /* [B, Hq, D] */

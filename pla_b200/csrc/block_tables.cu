@@ -17,7 +17,8 @@ constexpr int TPB = 256;          // threads, and new tokens, per CTA
 constexpr int PER = 4;            // requests per thread and scan
 constexpr int CHUNK = TPB * PER;
 
-__global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_tables_args p) {
+__global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_tables_args p, const Divisor page_size) {
+  auto pages = [&](int n) { return n > 0 ? page_size.quotient(n - 1) + 1 : 0; };      // that n tokens fill
   __shared__ int32_t s_off[CHUNK + 1];     // offsets of the chunk's requests
   __shared__ int32_t s_ctx[CHUNK];         // tokens in the cache; -1: bad metadata, no slots
   __shared__ int64_t s_base[CHUNK];        // first entry of the free list that the request takes
@@ -26,7 +27,6 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
   const int t0 = blockIdx.x * TPB;
   const int t = t0 + tid;
   const bool first_cta = blockIdx.x == 0;  // writes what there is per request
-  const int64_t bs = p.block_size;
   const int64_t start = p.free_start != nullptr ? max(*p.free_start, 0) : 0;
   int64_t running = start;
   int64_t slot = -1, pos = 0;
@@ -34,7 +34,8 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
   for (int n0 = 0; n0 < p.N; n0 += CHUNK) {
     const int cnt = min(CHUNK, p.N - n0);
     int32_t off[PER + 1], ctx[PER];
-    int64_t need[PER], mine = 0;
+    int need[PER];
+    int64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int n = n0 + tid * PER + i;
@@ -53,8 +54,8 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
         if (first_cta) p.seq_lens[n] = max(ctx[i], 0);
         s_ctx[tid * PER + i] = -1;
       } else {
-        const int64_t held = (ctx[i] + bs - 1) / bs, all = (ctx[i] + m + bs - 1) / bs;
-        need[i] = max(min(all, static_cast<int64_t>(p.columns)) - held, static_cast<int64_t>(0));
+        const int all = pages(ctx[i] + static_cast<int>(m));
+        need[i] = max(min(all, p.columns) - pages(ctx[i]), 0);
         if (all > p.columns) bad |= PLA_B200_DEV_TABLE_FULL;
         if (first_cta) p.seq_lens[n] = static_cast<int32_t>(ctx[i] + m);
         s_ctx[tid * PER + i] = ctx[i];
@@ -92,10 +93,10 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
         const int mid = (a + b) >> 1;
         if (s_off[mid] <= t) a = mid; else b = mid;
       }
-      const int64_t c = s_ctx[a], in = t - s_off[a];
-      if (c >= 0 && in >= 0 && t < s_off[a + 1]) {
-        pos = c + in;
-        const int64_t col = pos / bs, held = (c + bs - 1) / bs;
+      const int c = s_ctx[a];
+      if (c >= 0 && t >= s_off[a] && t < s_off[a + 1]) {
+        const int at_token = c + (t - s_off[a]), col = page_size.quotient(at_token), held = pages(c), in_page = at_token - col * p.block_size;
+        pos = at_token;
         if (col < p.columns) {
           int32_t* entry = p.block_table + (n0 + a) * p.table_row_stride + col;
           int32_t page = -1;
@@ -104,13 +105,14 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
           } else {
             const int64_t at = s_base[a] + col - held;
             if (at < p.free_count) page = p.free_blocks[at]; else bad |= PLA_B200_DEV_NO_BLOCK;
-            if (pos % bs == 0) *entry = page;
+            if (in_page == 0) *entry = page;
           }
-          if (page >= 0) slot = page * bs + pos % bs;
+          if (page >= 0) slot = static_cast<int64_t>(page) * p.block_size + in_page;
         }
       }
     }
     running += total;
+    if (first_cta && n0 + cnt == p.N && hi > p.tokens) bad |= PLA_B200_DEV_BAD_INTERVAL;    // rows that the caller has no room for
     if (!first_cta && lo > t0 + TPB - 1) break;     // the tile's tokens lie behind us
     __syncthreads();                       // the next chunk overwrites the shared arrays
   }
@@ -141,7 +143,7 @@ extern "C" int pla_b200_block_tables(const pla_b200_block_tables_args* args, voi
               "block_table rows must not overlap");
   PLA_REQUIRE(a.free_count == 0 || a.free_blocks, PLA_B200_E_INVALID, "free_blocks is NULL");
   const unsigned grid = static_cast<unsigned>(a.tokens > 0 ? (a.tokens + TPB - 1) / TPB : 1);
-  block_tables_kernel<<<grid, TPB, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  block_tables_kernel<<<grid, TPB, 0, static_cast<cudaStream_t>(stream)>>>(a, Divisor(static_cast<uint32_t>(a.block_size)));
   PLA_CUDA_OK(cudaGetLastError());
   return PLA_B200_OK;
 }

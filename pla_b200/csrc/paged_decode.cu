@@ -13,11 +13,16 @@
 // shared memory filled; in a unit each of the four other warps takes 16 tokens and keeps its own maxima, sums and output, without a
 // barrier between them until the range leaves the (request, head). Where pages hold whole tiles of 16 tokens, a tile is a box of a
 // tensor map over the cache, one copy per 64 channels; other page sizes take 16-byte asynchronous copies from each row's page. Both
-// leave the 128-byte swizzle that ldmatrix reads without bank conflicts. Tried before: one bulk copy per row and lane (the lanes'
-// copies issue one after another, 480 of 620 instructions per tile) and every warp loading for itself (240 instructions per tile
-// where this takes XXX; shorter heads and contexts are bound by them).
+// leave the 128-byte swizzle that ldmatrix reads without bank conflicts. Tried before: one bulk copy per row and lane (the lanes' copies
+// issue one after another, 480 of 620 instructions per tile of 16 tokens) and every warp loading for itself (290 per tile, here 240).
 // A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
-// waits on the first one's end only, joins the parts in order: no atomics, the same bits every time.
+// waits on the first one's end only, joins the parts in order: no atomics, the same bits every time. Calls with little work go to
+// clusters instead, which join their parts through distributed shared memory in the same kernel.
+// Device time on a B200: 64 requests up to 16K tokens, 16/2 heads of 256 (1.14 GB) 177 us, 6.4 TB/s; one of 128K, 32/8 heads of 128 (0.54 GB)
+// 91 us, 5.9 TB/s; 250 up to 2K, 32/4 heads of 64 (0.28 GB) 58 us, 4.9 TB/s; 8 up to 4K, 32/8 of 128 (71 MB) 21 us; one of 777, 16/2 of 128 5.4 us.
+// What is left: about 5 us until a CTA's first rows arrive (lengths, page table and rows are three reads that depend on each other), 10 %
+// between the first and the last CTA to finish (SMs get unequal shares of the bandwidth), and 4 us for the join. Handing out the last
+// eighth or quarter of the units from a counter evened the CTAs out, but the additional parts cost the join more (91 -> 109 us for 128K).
 // Scores, sums and outputs are 32-bit; the weights p are rounded to the activations' type for the product with V (relative 2^-8
 // or 2^-11, the same size as the output's own rounding), the sum of the weights is of the unrounded ones.
 #include <cuda.h>
@@ -784,9 +789,12 @@ int cache_map(CUtensorMap* map, const pla_b200_paged_decode_args& a, void* base,
                               static_cast<cuuint64_t>(a.num_blocks)};
   const cuuint64_t stride[3] = {bytes(a.Hk, st.head), bytes(a.block_size, st.token), bytes(a.num_blocks, st.block)};
   const cuuint32_t box[4] = {64, 1, TILE, 1}, step[4] = {1, 1, 1, 1};
+  // Rows of whole 256-byte pieces are fetched in these (one request of 128K tokens of 128 channels 93.5 -> 91.4 us); others would
+  // bring a neighbour's bytes along (D = 192: 81.3 -> 82.8 us).
+  const CUtensorMapL2promotion fetch = a.D % 128 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
   const CUresult rc = reinterpret_cast<Encode>(fn)(
       map, a.act_dtype == PLA_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, size, stride, box, step,
-      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PLA_REQUIRE(rc == CUDA_SUCCESS, PLA_B200_E_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(rc));
   return PLA_B200_OK;
 }

@@ -21,6 +21,11 @@ import torch
 
 from ..._ops import ops
 
+# the overloads themselves: half a microsecond less per call than looking them up through their packets
+_block_tables = ops.build_block_tables.default
+_rotary = ops.qk_rotary.default
+_paged_decode = ops.paged_attention_decode.default
+
 __all__ = [
     "BlockPlan",
     "apply_rotary",
@@ -61,9 +66,9 @@ def build_block_tables(
     -1 and position 0. Pass ``free_next`` as the next step's ``free_start`` to go on in the same list.
 
     ``status`` (int32[1]) gets 32 when the list ran out and 64 when a row has too few columns (the tokens without a page
-    have slot -1), 1 for negative lengths.
+    have slot -1), 1 for negative lengths and for offsets past ``num_tokens``.
     """
-    slots, positions, seq_lens, free_next = ops.build_block_tables(
+    slots, positions, seq_lens, free_next = _block_tables(
         block_table, context_lens, query_start_loc, free_blocks, block_size, num_tokens, free_start, status)
     return BlockPlan(block_table, slots, positions, seq_lens, free_next)
 
@@ -143,7 +148,7 @@ def apply_rotary(
     """Rotates the first ``2 * len(inv_freq)`` channels of every head of ``q`` ``[tokens, heads, dim]`` and ``k``
     by ``positions[t] * inv_freq`` and multiplies them by ``factor``; the other channels are copied. Pairs are ``(i, i + R/2)``, or
     ``(2i, 2i + 1)`` with ``interleaved``. ``out_q=q`` / ``out_k=k`` rotate in place."""
-    return ops.qk_rotary(q, k, None, None, None, positions, inv_freq, None, None, None, 0.0, factor, interleaved, False, out_q, out_k, None)
+    return _rotary(q, k, None, None, None, positions, inv_freq, None, None, None, 0.0, factor, interleaved, False, out_q, out_k, None)
 
 
 def qk_norm_rotary(
@@ -163,8 +168,8 @@ def qk_norm_rotary(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """RMS norm of every head of ``q`` and ``k`` (``x * rsqrt(mean(x^2) + eps) * weight``, ``1 + weight`` with ``unit_offset``; a
     ``None`` weight leaves that side as it is), then the rotation of :func:`apply_rotary`, in one pass."""
-    return ops.qk_rotary(q, k, None, q_weight, k_weight, positions, inv_freq, None, None, None, eps, factor, interleaved, unit_offset, out_q,
-                         out_k, None)
+    return _rotary(q, k, None, q_weight, k_weight, positions, inv_freq, None, None, None, eps, factor, interleaved, unit_offset, out_q, out_k,
+                   None)
 
 
 def qk_norm_rotary_cache(
@@ -189,8 +194,8 @@ def qk_norm_rotary_cache(
     """:func:`qk_norm_rotary` whose keys go to ``k_cache[slot // block_size, slot % block_size]`` (``[blocks, block_size, kv heads, dim]``
     with any strides) and whose values are copied to ``v_cache`` likewise; returns the queries. A negative slot stores
     nothing; a slot outside the pool stores nothing and sets 8 in ``status``. The slots of a call must differ."""
-    return ops.qk_rotary(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
-                         unit_offset, out_q, None, status)[0]
+    return _rotary(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
+                   unit_offset, out_q, None, status)[0]
 
 
 def paged_attention_decode(
@@ -212,5 +217,5 @@ def paged_attention_decode(
 
     ``status`` (int32[1]) gets 1 for a length that is negative or past the table's row, 8 for a page outside the pool (its
     tokens are left out)."""
-    o, lse = ops.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, return_lse, status)
+    o, lse = _paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, return_lse, status)
     return (o, lse) if return_lse else o

@@ -188,6 +188,10 @@ def test_tables_edges(native_built):
     tables_case([2] * 40, [1] * 40, 4, free=0)                                    # no list at all: only pages that are held
     plan = fa().build_block_tables(torch.empty(0, 4, dtype=torch.int32, device="cuda"), i32([]), i32([0]), i32([3]), 4, num_tokens=3)
     assert plan.slot_mapping.tolist() == [-1] * 3 and plan.positions.tolist() == [0] * 3 and plan.free_next.tolist() == [0]
+    # offsets past the token rows: the rest is left out, flagged
+    table, status = torch.full((2, 3), -7, dtype=torch.int32, device="cuda"), word()
+    plan = fa().build_block_tables(table, i32([0, 0]), i32([0, 2, 9]), i32([5, 6, 7]), 4, num_tokens=3, status=status)
+    assert status.item() == 1 and plan.slot_mapping.tolist() == [20, 21, 24] and table.tolist() == [[5, -7, -7], [6, -7, -7]]
     # offsets that decrease: the request takes nothing and nothing is written out of place
     table, status = torch.full((2, 3), -7, dtype=torch.int32, device="cuda"), word()
     plan = fa().build_block_tables(table, i32([0, 0]), i32([0, 4, 2]), i32([5, 6]), 4, num_tokens=4, status=status)
