@@ -57,7 +57,7 @@ int pla_b200_block_tables(const pla_b200_block_tables_args* args, void* stream);
  *   y = x * rsqrt(mean(x^2) + eps) * (w + unit_offset)           (when the weight is given)
  *   (y_a, y_b) <- factor * (y_a cos - y_b sin, y_b cos + y_a sin),  angle = position * inv_freq[i]
  * with (a, b) = (i, i + R/2), or (2i, 2i + 1) when interleaved. Angles are reduced to one turn in 64 bits; one rounding at the end.
- * k may be absent (Hk = 0). With k_cache, k rows go to their slots instead of (or besides) k_out, and v rows
+ * k may be absent (Hk = 0). With k_cache (then k_out is NULL), k rows go to their slots and v rows
  * are copied to theirs; a slot < 0 stores nothing, a slot outside the pool sets PLA_B200_DEV_BAD_SLOT. Slots of one call
  * must differ. q_out / k_out may be q / k themselves. Rows and strides are multiples of 16 bytes.
  * ======================================================================== */
@@ -67,7 +67,7 @@ typedef struct pla_b200_rotary_args {
   const void* v;       /* [T, Hk, D], with k_cache */
   int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
   void* q_out;
-  void* k_out;         /* may be NULL with k_cache */
+  void* k_out;         /* NULL with k_cache */
   int64_t qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride;
   const void* q_weight; /* [D] or NULL (no norm of q) */
   const void* k_weight; /* [D] or NULL (no norm of k) */

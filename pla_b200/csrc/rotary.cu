@@ -13,8 +13,8 @@
 // 16-byte asynchronous copies into cells that only the copying lane reads.
 // On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 109 us, 6.1 TB/s; rotation alone of 32,761
 // tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 123 us, 5.5 TB/s; 1,999 tokens with the norm (41 MB) 13 us; one token 3 us. At 2.6
-// instructions per cycle and SM the arithmetic alone takes about 75 us of these, so latency and issue slots are what is left. Measured
-// and not kept: two channels per instruction (fma.f32x2; the register pairs cost more moves than it saves, 61 -> 83 million instructions for
+// instructions per cycle and SM the arithmetic alone takes about 75 us of these; a seventh fewer instructions did not shorten the large
+// calls, so what is left is how well reads and writes overlap. Measured and not kept: two channels per instruction (fma.f32x2; the register pairs cost more moves than it saves, 61 -> 83 million instructions for
 // the interleaved case), three CTAs per SM (80 registers spill, 167 us), 64-bit floating-point angles (the wrapped integers are exact and
 // a few percent faster).
 #include "common.cuh"
@@ -260,14 +260,15 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) rotary_kernel(const __grid
             cached += cache_step;
           }
           issue(cell);
-          cell = cell + 1 == RING ? 0 : cell + 1;
+          cell = (cell + 1) & (RING - 1);
           h += ROWS;
         }
         break;
       }
       const bool normed = z.weight != nullptr, dense = z.out != nullptr;
-      act_t* out = static_cast<act_t*>(z.out) + e[0] + wide(t, z.out_tok) + wide(h, z.out_head);
-      const int64_t out_step = wide(ROWS, z.out_head);
+      act_t* out = dense ? static_cast<act_t*>(z.out) + e[0] + wide(t, z.out_tok) + wide(h, z.out_head) : cached;
+      const int64_t out_step = dense ? wide(ROWS, z.out_head) : cache_step;
+      const bool stored = out != nullptr;              // not: keys of a padding row
 
       // weights, sines and cosines of the lane's channels
       float A[2][8], B[2][8];
@@ -426,20 +427,18 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) rotary_kernel(const __grid
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i / 8][i % 8] *= inv;
         }
-        if (h < heads) {
+        if (h < heads && stored) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (!on[c]) continue;
             const uint4 packed = pack<act_t>(y[c]);
-            if (dense) *reinterpret_cast<uint4*>(out + c * upper) = packed;
-            if (cached != nullptr) *reinterpret_cast<uint4*>(cached + c * upper) = packed;
+            *reinterpret_cast<uint4*>(out + c * upper) = packed;
           }
         }
         issue(cell);
-        cell = cell + 1 == RING ? 0 : cell + 1;
+        cell = (cell + 1) & (RING - 1);
         h += ROWS;
         out += out_step;
-        if (cached != nullptr) cached += cache_step;
       }
     }
     __syncwarp();                          // the next token overwrites sines and cosines
@@ -517,6 +516,7 @@ extern "C" int pla_b200_rotary(const pla_b200_rotary_args* args, void* stream) {
     PLA_REQUIRE(stride >= 0 && stride <= INT32_MAX, PLA_B200_E_TOO_LARGE, "token and head strides must be below 2^31 elements");
   PLA_REQUIRE(a.Hq < 65536 && a.Hk < 65536, PLA_B200_E_TOO_LARGE, "too many heads");
   if (a.k_cache != nullptr) {
+    PLA_REQUIRE(a.k_out == nullptr, PLA_B200_E_INVALID, "keys go either to k_out or to the cache");
     PLA_REQUIRE(a.v_cache && a.v && a.slots.data && a.num_blocks >= 0 && a.block_size > 0, PLA_B200_E_INVALID,
                 "a cache needs k_cache, v_cache, v, slots, num_blocks >= 0 and block_size > 0");
     PLA_REQUIRE(aligned16(a.k_cache) && aligned16(a.v_cache) && aligned16(a.v) && strides16(a.k_strides) && strides16(a.v_strides) &&
