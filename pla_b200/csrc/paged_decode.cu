@@ -27,6 +27,8 @@
 // or 2^-11, the same size as the output's own rounding), the sum of the weights is of the unrounded ones.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "../../include/pla_b200_attention.h"
 
@@ -118,7 +120,10 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
                ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(token), "r"(page), "r"(smem_addr(bar))
                : "memory");
 }
-// 16 bytes from global memory, or zeros.
+// 16 bytes from global memory; or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
@@ -203,6 +208,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
   __shared__ uint64_t s_full[STAGES], s_free[STAGES];
   __shared__ uint16_t s_live[STAGES][WARPS];       // rows of each tile that hold a token
   __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
+  __shared__ const void* s_rows[BOXED ? 1 : 2][BOXED ? 1 : UNIT];
   __shared__ int64_t s_scan[WARPS + 1];
   __shared__ int s_place[4];
   __shared__ float s_part_m[8 * NT], s_part_l[8 * NT];    // TEAMED: the CTA's part; its sums take the ring's place at the end
@@ -351,29 +357,52 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           for (int c = 0; c < S::BOXES; ++c) load_box(row + S::ROWS + c * S::BOX, &v_map, c * 64, head, in[0], from[0], bar);
         }
       } else {
+        // Row addresses go through shared memory; then a lane keeps one 16-byte column and takes every RPS-th row of it.
+        constexpr int COLUMNS = D / 8, RPS = 32 / COLUMNS;                // lanes past RPS * COLUMNS have none (D = 96, 192)
         uint32_t rows[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) rows[u] = __ballot_sync(0xffffffffu, live[u]);
+        for (int u = 0; u < 2; ++u) {
+          rows[u] = __ballot_sync(0xffffffffu, live[u]);
+          const act_t *k_row = static_cast<const act_t*>(p.q), *v_row = k_row;    // a valid address for rows that are not read
+          if (live[u]) {
+            k_row = static_cast<const act_t*>(p.k_cache) + from[u] * p.k_strides.block + in[u] * p.k_strides.token + head * p.k_strides.head;
+            v_row = static_cast<const act_t*>(p.v_cache) + from[u] * p.v_strides.block + in[u] * p.v_strides.token + head * p.v_strides.head;
+          }
+          s_rows[0][lane + u * 32] = k_row;
+          s_rows[1][lane + u * 32] = v_row;
+        }
         if (lane < WARPS) s_live[stage][lane] = static_cast<uint16_t>(rows[lane >> 1] >> ((lane & 1) * 16));
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
+        const int c = lane % COLUMNS, sub = lane / COLUMNS;
+        if (sub < RPS) {
+          // row r of the column sits at r * 128 + (((c & 7) ^ (r & 7)) << 4); r = sub + a multiple of RPS, whose bits are apart
+          const uint32_t dst = to + (c >> 3) * S::BOX + sub * 128, swizzle = ((c & 7) ^ sub) << 4;
+          constexpr int AHEAD = 8;                                        // addresses read before their copies are issued
+          auto bring = [&](auto all) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < UNIT; r0 += AHEAD * RPS) {
+              const act_t* at_row[2][AHEAD];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {                            // keys, values
-          const pla_b200_page_strides st = side ? p.v_strides : p.k_strides;
-          const act_t* const base = static_cast<const act_t*>(side ? p.v_cache : p.k_cache);
+              for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const act_t* src = static_cast<const act_t*>(p.q);            // a valid address for rows that are not read
-            if (live[u]) src = base + from[u] * st.block + in[u] * st.token + head * st.head;
-#pragma unroll 4
-            for (int k = lane; k < 32 * (D / 8); k += 32) {
-              const int r = k / (D / 8), c = k % (D / 8);                 // r: the lane that knows the row
-              const act_t* row = reinterpret_cast<const act_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r));
-              copy16(to + side * S::ROWS + (c >> 3) * S::BOX + (u * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), row + c * 8, (rows[u] >> r) & 1);
+                for (int side = 0; side < 2; ++side) at_row[side][u] = static_cast<const act_t*>(s_rows[side][r0 + u * RPS + sub]) + c * 8;
+              const uint32_t here = rows[r0 >> 5] >> ((r0 & 31) + sub);               // AHEAD * RPS divides 32
+#pragma unroll
+              for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                  const uint32_t at = dst + side * S::ROWS + (r0 + u * RPS) * 128 + (swizzle ^ (((r0 + u * RPS) & 7) << 4));
+                  if constexpr (all.value) copy16(at, at_row[side][u]);
+                  else copy16(at, at_row[side][u], (here >> (u * RPS)) & 1);
+                }
             }
-          }
+          };
+          if ((rows[0] & rows[1]) == 0xffffffffu) bring(std::true_type{});
+          else bring(std::false_type{});
         }
         copies_arrive(bar);
+        __syncwarp();                                                     // s_rows is written again
       }
     }
     if (timed_out) bad |= PLA_B200_DEV_WAIT_TIMEOUT;
