@@ -36,7 +36,7 @@ namespace pla {
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int THREADS = WARPS * 32;   // of the warps that compute; one more loads
+constexpr int THREADS = WARPS * 32;   // of the warps that compute; producers come on top
 constexpr int TILE = 16;              // tokens per warp and step
 constexpr int UNIT = TILE * WARPS;    // tokens per CTA and step
 constexpr float LOG2E = 1.4426950408889634f;
@@ -194,22 +194,26 @@ __device__ __forceinline__ float4 team_load4(uint32_t addr) {
   return x;
 }
 
+// Warps that load: rows one by one take two where the registers allow it (they are few with three CTAs per SM).
+template <int D, bool BOXED>
+constexpr int LOADERS = BOXED || D == 64 ? 1 : 2;
+
 // BOXED: pages hold whole tiles, the maps describe the caches. TEAMED: the calls with little work. A cluster of TEAM CTAs takes one
 // (request, head), each CTA an equal range of its units, and they join their parts through distributed shared memory: no lengths to add
 // up, no workspace, no second kernel.
 template <typename act_t, int D, int NT, bool BOXED, bool TEAMED>
-__global__ void __launch_bounds__(THREADS + 32, Shape<D>::CTAS)
+__global__ void __launch_bounds__(THREADS + 32 * LOADERS<D, BOXED>, Shape<D>::CTAS)
 paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D>;
-  constexpr int STAGES = S::STAGES;
+  constexpr int STAGES = S::STAGES, PRODUCERS = LOADERS<D, BOXED>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   __shared__ uint64_t s_full[STAGES], s_free[STAGES];
   __shared__ uint16_t s_live[STAGES][WARPS];       // rows of each tile that hold a token
   __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
   __shared__ const void* s_rows[BOXED ? 1 : 2][BOXED ? 1 : UNIT];
-  __shared__ int64_t s_scan[WARPS + 1];
+  __shared__ int64_t s_scan[WARPS + PRODUCERS];
   __shared__ int s_place[4];
   __shared__ float s_part_m[8 * NT], s_part_l[8 * NT];    // TEAMED: the CTA's part; its sums take the ring's place at the end
   if (!TEAMED) asm volatile("griddepcontrol.launch_dependents;");
@@ -224,7 +228,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
   // ---- the CTA's range of units
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&s_full[i], BOXED ? 1 : 33);       // the producer's lane 0, and every lane's copies
+      mbar_init(&s_full[i], BOXED ? 1 : 33 * PRODUCERS);       // a producer's lane 0, and every lane's copies
       mbar_init(&s_free[i], WARPS);
     }
     fence_mbar_init();
@@ -269,7 +273,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
     }
     if (lane == 31) s_scan[warp] = upto;
     __syncthreads();
-    for (int w = 0; w <= WARPS; ++w) {
+    for (int w = 0; w < WARPS + PRODUCERS; ++w) {
       if (w < warp) upto += s_scan[w];
       total += s_scan[w];
     }
@@ -310,13 +314,14 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
 
   const uint32_t ring = smem_addr(smem);
   bool timed_out = false;
-  if (warp == WARPS) {
-    // ---- producer: token of the lane, that of tile lane % 4 when tiles come as boxes, else those of rows lane and lane + 32
+  if (warp >= WARPS) {
+    // ---- producer: token of the lane, that of tile lane % 4 when tiles come as boxes, else of every 32nd of its rows
     auto page_of = [&](int t) -> int {               // -1 past the end
       return t < at.len ? p.block_table[at.b * p.table_row_stride + plan.page.quotient(t)] : -1;
     };
-    constexpr int TOKENS = BOXED ? 1 : 2;
-    auto token = [&](int u) { return at.unit * UNIT + (BOXED ? (lane & 3) * TILE : lane + u * 32); };
+    constexpr int TOKENS = BOXED ? 1 : 2 / PRODUCERS;
+    const int first_row = BOXED ? 0 : (warp - WARPS) * TOKENS * 32;       // of the producer's
+    auto token = [&](int u) { return at.unit * UNIT + (BOXED ? (lane & 3) * TILE : first_row + u * 32 + lane); };
     int page[TOKENS];
 #pragma unroll
     for (int u = 0; u < TOKENS; ++u) page[u] = page_of(token(u));
@@ -359,19 +364,19 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
       } else {
         // Row addresses go through shared memory; then a lane keeps one 16-byte column and takes every RPS-th row of it.
         constexpr int COLUMNS = D / 8, RPS = 32 / COLUMNS;                // lanes past RPS * COLUMNS have none (D = 96, 192)
-        uint32_t rows[2];
+        uint32_t rows[TOKENS];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < TOKENS; ++u) {
           rows[u] = __ballot_sync(0xffffffffu, live[u]);
           const act_t *k_row = static_cast<const act_t*>(p.q), *v_row = k_row;    // a valid address for rows that are not read
           if (live[u]) {
             k_row = static_cast<const act_t*>(p.k_cache) + from[u] * p.k_strides.block + in[u] * p.k_strides.token + head * p.k_strides.head;
             v_row = static_cast<const act_t*>(p.v_cache) + from[u] * p.v_strides.block + in[u] * p.v_strides.token + head * p.v_strides.head;
           }
-          s_rows[0][lane + u * 32] = k_row;
-          s_rows[1][lane + u * 32] = v_row;
+          s_rows[0][first_row + u * 32 + lane] = k_row;
+          s_rows[1][first_row + u * 32 + lane] = v_row;
         }
-        if (lane < WARPS) s_live[stage][lane] = static_cast<uint16_t>(rows[lane >> 1] >> ((lane & 1) * 16));
+        if (lane < 2 * TOKENS) s_live[stage][first_row / TILE + lane] = static_cast<uint16_t>(rows[lane >> 1] >> ((lane & 1) * 16));
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
         const int c = lane % COLUMNS, sub = lane / COLUMNS;
@@ -381,13 +386,13 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           constexpr int AHEAD = 8;                                        // addresses read before their copies are issued
           auto bring = [&](auto all) {
 #pragma unroll 1
-            for (int r0 = 0; r0 < UNIT; r0 += AHEAD * RPS) {
+            for (int r0 = first_row; r0 < first_row + TOKENS * 32; r0 += AHEAD * RPS) {
               const act_t* at_row[2][AHEAD];
 #pragma unroll
               for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
                 for (int side = 0; side < 2; ++side) at_row[side][u] = static_cast<const act_t*>(s_rows[side][r0 + u * RPS + sub]) + c * 8;
-              const uint32_t here = rows[r0 >> 5] >> ((r0 & 31) + sub);               // AHEAD * RPS divides 32
+              const uint32_t here = rows[TOKENS - 1 && (r0 & 32)] >> ((r0 & 31) + sub);   // AHEAD * RPS divides 32
 #pragma unroll
               for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
@@ -398,7 +403,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
                 }
             }
           };
-          if ((rows[0] & rows[1]) == 0xffffffffu) bring(std::true_type{});
+          if ((rows[0] & rows[TOKENS - 1]) == 0xffffffffu) bring(std::true_type{});
           else bring(std::false_type{});
         }
         copies_arrive(bar);
@@ -870,7 +875,7 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   if constexpr (TEAMED) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.grid);
-    cfg.blockDim = dim3(THREADS + 32);
+    cfg.blockDim = dim3(THREADS + 32 * LOADERS<D, BOXED>);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -882,7 +887,7 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
     PLA_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_kernel<act_t, D, NT, BOXED, TEAMED>, a, plan, k_map, v_map));
     return PLA_B200_OK;
   }
-  paged_decode_kernel<act_t, D, NT, BOXED, TEAMED><<<plan.grid, THREADS + 32, S::SMEM, stream>>>(a, plan, k_map, v_map);
+  paged_decode_kernel<act_t, D, NT, BOXED, TEAMED><<<plan.grid, THREADS + 32 * LOADERS<D, BOXED>, S::SMEM, stream>>>(a, plan, k_map, v_map);
   PLA_CUDA_OK(cudaGetLastError());
   if (units_of_row(a) > 1) {                        // else every item is one unit and was stored whole
     cudaLaunchConfig_t cfg = {};
