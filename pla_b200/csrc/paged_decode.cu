@@ -12,7 +12,8 @@
 // the lengths are and splits a single long request over all of them. A producer warp walks the range and keeps a ring of units in
 // shared memory filled; in a unit each of the four other warps takes 16 tokens and keeps its own maxima, sums and output, without a
 // barrier between them until the range leaves the (request, head). Where pages hold whole tiles of 16 tokens, a tile is a box of a
-// tensor map over the cache, one copy per 64 channels; other page sizes take 16-byte asynchronous copies from each row's page. Both
+// tensor map over the cache, one copy per 64 channels; other page sizes take two producer warps and 16-byte asynchronous copies from
+// each row's page (32 requests up to 8K tokens of 8 heads of 128: 93 us in pages of one token, 85 is the floor). Both
 // leave the 128-byte swizzle that ldmatrix reads without bank conflicts. Tried before: one bulk copy per row and lane (the lanes' copies
 // issue one after another, 480 of 620 instructions per tile of 16 tokens) and every warp loading for itself (290 per tile, here 240).
 // A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
@@ -194,19 +195,20 @@ __device__ __forceinline__ float4 team_load4(uint32_t addr) {
   return x;
 }
 
-// Warps that load: rows one by one take two where the registers allow it (they are few with three CTAs per SM).
-template <int D, bool BOXED>
-constexpr int LOADERS = BOXED || D == 64 ? 1 : 2;
+// Warps that load: rows one by one take two (64 requests up to 8K tokens of 4 heads of 64 67 -> 59 us, of 2 heads of 256 137 -> 98), except
+// where the computing warps need the registers (16 query heads of 64, three CTAs per SM: 41.8 us with one, 43.9 with two).
+template <int D, int NT, bool BOXED>
+constexpr int LOADERS = BOXED || (D == 64 && NT == 2) ? 1 : 2;
 
 // BOXED: pages hold whole tiles, the maps describe the caches. TEAMED: the calls with little work. A cluster of TEAM CTAs takes one
 // (request, head), each CTA an equal range of its units, and they join their parts through distributed shared memory: no lengths to add
 // up, no workspace, no second kernel.
 template <typename act_t, int D, int NT, bool BOXED, bool TEAMED>
-__global__ void __launch_bounds__(THREADS + 32 * LOADERS<D, BOXED>, Shape<D>::CTAS)
+__global__ void __launch_bounds__(THREADS + 32 * LOADERS<D, NT, BOXED>, Shape<D>::CTAS)
 paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D>;
-  constexpr int STAGES = S::STAGES, PRODUCERS = LOADERS<D, BOXED>;
+  constexpr int STAGES = S::STAGES, PRODUCERS = LOADERS<D, NT, BOXED>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
   __shared__ uint64_t s_full[STAGES], s_free[STAGES];
@@ -875,7 +877,7 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
   if constexpr (TEAMED) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.grid);
-    cfg.blockDim = dim3(THREADS + 32 * LOADERS<D, BOXED>);
+    cfg.blockDim = dim3(THREADS + 32 * LOADERS<D, NT, BOXED>);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -887,7 +889,7 @@ int launch(const pla_b200_paged_decode_args& a, cudaStream_t stream) {
     PLA_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_kernel<act_t, D, NT, BOXED, TEAMED>, a, plan, k_map, v_map));
     return PLA_B200_OK;
   }
-  paged_decode_kernel<act_t, D, NT, BOXED, TEAMED><<<plan.grid, THREADS + 32 * LOADERS<D, BOXED>, S::SMEM, stream>>>(a, plan, k_map, v_map);
+  paged_decode_kernel<act_t, D, NT, BOXED, TEAMED><<<plan.grid, THREADS + 32 * LOADERS<D, NT, BOXED>, S::SMEM, stream>>>(a, plan, k_map, v_map);
   PLA_CUDA_OK(cudaGetLastError());
   if (units_of_row(a) > 1) {                        // else every item is one unit and was stored whole
     cudaLaunchConfig_t cfg = {};

@@ -438,7 +438,8 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 257, 700]
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("hq,hk,D,bs,layout", [(16, 2, 256, 16, "separate"), (32, 8, 128, 16, "packed"), (8, 8, 64, 1, "heads"), (5, 1, 96, 7, "separate"),
                                                (12, 2, 192, 48, "heads"), (16, 1, 128, 64, "packed"), (3, 1, 256, 128, "heads"), (40, 2, 64, 32, "separate"),
-                                               (33, 1, 128, 16, "separate"), (34, 2, 256, 16, "heads")])
+                                               (33, 1, 128, 16, "separate"), (34, 2, 256, 16, "heads"), (16, 2, 256, 7, "heads"), (8, 8, 128, 1, "packed"),
+                                               (6, 2, 192, 20, "separate"), (128, 2, 64, 8, "packed"), (18, 1, 256, 1, "separate")])
 def test_attention_matches_the_oracle(native_built, hq, hk, D, bs, layout, dtype):
     q, kc, vc, table = paged_inputs(hq * D + bs, EDGES, hq, hk, D, bs, DT[dtype], layout)
     status = word()
@@ -452,8 +453,10 @@ def test_attention_matches_the_oracle(native_built, hq, hk, D, bs, layout, dtype
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens,hq,hk,D,bs", [([5000], 16, 2, 128, 16), ([9001, 3, 0, 1200], 8, 1, 256, 64), ([4096] * 3, 4, 4, 64, 32), ([0, 0], 4, 2, 128, 16),
-                                             ([1], 1, 1, 64, 1), ([40] * 300, 8, 2, 64, 16), ([1] * 700, 4, 4, 96, 16)],
-                         ids=["one-5000", "ragged-9001", "even-4096", "all-empty", "one-token", "300x40", "700x1"])
+                                             ([1], 1, 1, 64, 1), ([40] * 300, 8, 2, 64, 16), ([1] * 700, 4, 4, 96, 16), ([i % 5 for i in range(3000)], 2, 1, 64, 4),
+                                             ([20011, 7], 4, 1, 192, 9), ([12000, 300, 0, 5], 2, 2, 128, 1), ([64] * 40, 8, 8, 128, 64)],
+                         ids=["one-5000", "ragged-9001", "even-4096", "all-empty", "one-token", "300x40", "700x1", "3000-tiny", "rows-20011",
+                              "rows-12000", "one-unit-rows"])
 def test_attention_lengths(native_built, lens, hq, hk, D, bs):
     q, kc, vc, table = paged_inputs(len(lens) + D, lens, hq, hk, D, bs)
     out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), return_lse=True, scale=0.11)
