@@ -199,6 +199,31 @@ def test_tables_edges(native_built):
 
 
 @pytest.mark.gpu
+def test_tables_with_many_requests_and_streams(native_built):
+    """More requests than one scan holds, several tiles of tokens; the same on another stream and replayed from a graph with other
+    lengths in the same tensors."""
+    context, new = [(i * 37) % 500 for i in range(5000)], [(i * 11) % 4 for i in range(5000)]
+    tables_case(context, new, 16)
+    table, ctx, off = torch.zeros(3, 8, dtype=torch.int32, device="cuda"), i32([0, 0, 0]), i32([0, 4, 8, 12])
+    free = i32(list(range(10, 40)))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        plan = fa().build_block_tables(table, ctx, off, free, 4, num_tokens=12)
+    side.synchronize()
+    assert plan.slot_mapping.tolist() == [4 * p + i for p in (10, 11, 12) for i in range(4)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan = fa().build_block_tables(table, ctx, off, free, 4, num_tokens=12)
+    for c, o in (([4, 3, 0], [0, 1, 2, 7]), ([0, 0, 8], [0, 0, 0, 1])):
+        rows = [[20 + 2 * r, 21 + 2 * r] + [0] * 6 for r in range(3)]
+        table.copy_(i32(rows)), ctx.copy_(i32(c)), off.copy_(i32(o))
+        g.replay()
+        want = ofa.block_tables(rows, c, o, free.tolist(), 4, 12)
+        assert plan.slot_mapping.tolist() == want[1] and table.tolist() == want[0] and plan.free_next.tolist() == [want[4]]
+
+
+@pytest.mark.gpu
 def test_tables_slots_past_32_bits(native_built):
     plan = fa().build_block_tables(i32([[-1]]), i32([0]), i32([0, 3]), i32([2 ** 31 - 1]), 1 << 20, num_tokens=3)
     base = (2 ** 31 - 1) << 20
@@ -579,6 +604,38 @@ def test_attention_cache_past_32_bit_offsets(native_built):
     slot = torch.tensor([(blocks - 3) * bs + 5], device="cuda")
     fa().qk_norm_rotary_cache(x, x, x, None, None, i32([0]), torch.ones(8, dtype=torch.float64, device="cuda"), big_k, big_v, slot)
     assert torch.equal(big_k[blocks - 3, 5], x[0]) and torch.equal(big_v[blocks - 3, 5], x[0])
+
+
+@pytest.mark.gpu
+def test_attention_through_the_abi(native_built):
+    """The C entry with a workspace that holds garbage; a missing, a too small and an unaligned one are refused."""
+    import ctypes
+    from pla_b200 import capi
+    lib = capi.load()
+    lens = [900, 0, 4100]
+    q, kc, vc, table = paged_inputs(21, lens, 16, 8, 128, 16)
+    dq, dt, dl, out, lse = q.cuda(), table.cuda(), i32(lens), torch.empty_like(q, device="cuda"), torch.empty(3, 16, device="cuda")
+    a = capi.pla_b200_paged_decode_args(q=dq.data_ptr(), q_row_stride=dq.stride(0), q_head_stride=dq.stride(1), k_cache=kc.data_ptr(),
+                                        v_cache=vc.data_ptr(), block_table=dt.data_ptr(), table_row_stride=dt.stride(0),
+                                        seq_lens=dl.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), num_blocks=kc.shape[0], block_size=16,
+                                        columns=dt.shape[1], B=3, Hq=16, Hk=8, D=128, act_dtype=0, scale=128 ** -0.5)
+    for name, x in (("k_strides", kc), ("v_strides", vc)):
+        st = getattr(a, name)
+        st.block, st.token, st.head = x.stride(0), x.stride(1), x.stride(2)
+    size = lib.pla_b200_paged_decode_workspace_bytes(ctypes.byref(a))
+    assert size > 0
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.pla_b200_paged_decode(ctypes.byref(a), stream) == -1 and b"workspace" in lib.pla_b200_last_error()
+    space = torch.full((size + 16,), 0xff, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = space.data_ptr(), size - 1
+    assert lib.pla_b200_paged_decode(ctypes.byref(a), stream) == -1
+    a.workspace, a.workspace_bytes = space.data_ptr() + 8, size
+    assert lib.pla_b200_paged_decode(ctypes.byref(a), stream) == -2
+    a.workspace = space.data_ptr()
+    assert lib.pla_b200_paged_decode(ctypes.byref(a), stream) == 0, lib.pla_b200_last_error()
+    torch.cuda.synchronize()
+    assert (space[size:] == 0xff).all()
+    assert_attention(out, lse, q, kc, vc, table, lens)
 
 
 @pytest.mark.gpu
