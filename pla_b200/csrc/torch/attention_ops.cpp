@@ -144,12 +144,12 @@ at::Tensor out_rows(const std::optional<at::Tensor>& out, const at::Tensor& like
   return *out;
 }
 
-std::tuple<at::Tensor, at::Tensor> qk_rotary(
+std::tuple<at::Tensor, at::Tensor> rotary(
     const at::Tensor& q, const std::optional<at::Tensor>& k, const std::optional<at::Tensor>& v,
     const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight, const at::Tensor& positions,
     const at::Tensor& inv_freq, const std::optional<at::Tensor>& k_cache, const std::optional<at::Tensor>& v_cache,
     const std::optional<at::Tensor>& slot_mapping, double eps, double factor, bool interleaved, bool unit_offset,
-    const std::optional<at::Tensor>& out_q, const std::optional<at::Tensor>& out_k, const std::optional<at::Tensor>& status) {
+    const std::optional<at::Tensor>& out_q, const std::optional<at::Tensor>& out_k, const std::optional<at::Tensor>& status, const char* op) {
   check_cuda(q, "q");
   const at::Device device = q.device();
   check_rows(q, device, "q");
@@ -222,15 +222,41 @@ std::tuple<at::Tensor, at::Tensor> qk_rotary(
   g.act_dtype = dtype_tag(q, "q");
   g.factor = static_cast<float>(factor);
   g.eps = static_cast<float>(eps);
-  if (!bypass_exec()) check_abi(pla_b200_rotary(&g, stream_of(q)), "qk_rotary");
+  if (!bypass_exec()) check_abi(pla_b200_rotary(&g, stream_of(q)), op);
   return {qo, ko};
+}
+
+// One operator per use: an argument costs about a tenth of a microsecond on its way through the dispatcher.
+std::tuple<at::Tensor, at::Tensor> apply_rotary(const at::Tensor& q, const std::optional<at::Tensor>& k, const at::Tensor& positions,
+                                                const at::Tensor& inv_freq, double factor, bool interleaved,
+                                                const std::optional<at::Tensor>& out_q, const std::optional<at::Tensor>& out_k) {
+  return rotary(q, k, std::nullopt, std::nullopt, std::nullopt, positions, inv_freq, std::nullopt, std::nullopt, std::nullopt, 0.0, factor,
+                interleaved, false, out_q, out_k, std::nullopt, "apply_rotary");
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const std::optional<at::Tensor>& k,
+                                                  const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight,
+                                                  const at::Tensor& positions, const at::Tensor& inv_freq, double eps, double factor,
+                                                  bool interleaved, bool unit_offset, const std::optional<at::Tensor>& out_q,
+                                                  const std::optional<at::Tensor>& out_k) {
+  return rotary(q, k, std::nullopt, q_weight, k_weight, positions, inv_freq, std::nullopt, std::nullopt, std::nullopt, eps, factor,
+                interleaved, unit_offset, out_q, out_k, std::nullopt, "qk_norm_rotary");
+}
+
+at::Tensor qk_norm_rotary_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& q_weight,
+                                const std::optional<at::Tensor>& k_weight, const at::Tensor& positions, const at::Tensor& inv_freq,
+                                const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& slot_mapping, double eps, double factor,
+                                bool interleaved, bool unit_offset, const std::optional<at::Tensor>& out_q,
+                                const std::optional<at::Tensor>& status) {
+  return std::get<0>(rotary(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
+                            unit_offset, out_q, std::nullopt, status, "qk_norm_rotary_cache"));
 }
 
 // ---------------------------------------------------------------------------------------------- paged decode
 std::tuple<at::Tensor, at::Tensor> paged_attention_decode(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                                                           const at::Tensor& block_table, const at::Tensor& seq_lens,
-                                                          std::optional<double> scale, const std::optional<at::Tensor>& out,
-                                                          bool return_lse, const std::optional<at::Tensor>& status) {
+                                                          std::optional<double> scale, bool return_lse,
+                                                          const std::optional<at::Tensor>& out, const std::optional<at::Tensor>& status) {
   check_cuda(q, "q");
   const at::Device device = q.device();
   TORCH_CHECK(q.dim() == 3, "q must have shape [requests, heads, dim]");
@@ -309,15 +335,23 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_decode(const at::Tensor& q, c
 TORCH_LIBRARY_FRAGMENT(pla_b200, m) {
   m.def(
       "build_block_tables(Tensor(a!) block_table, Tensor context_lens, Tensor query_start_loc, Tensor free_blocks, int block_size, "
-      "int num_tokens, Tensor? free_start, Tensor(b!)? status) -> (Tensor, Tensor, Tensor, Tensor)",
+      "int num_tokens, Tensor? free_start=None, Tensor(b!)? status=None) -> (Tensor, Tensor, Tensor, Tensor)",
       &pla_ops::build_block_tables);
   m.def(
-      "qk_rotary(Tensor q, Tensor? k, Tensor? v, Tensor? q_weight, Tensor? k_weight, Tensor positions, Tensor inv_freq, "
-      "Tensor(a!)? k_cache, Tensor(b!)? v_cache, Tensor? slot_mapping, float eps, float factor, bool interleaved, bool unit_offset, "
-      "Tensor(c!)? out_q, Tensor(d!)? out_k, Tensor(e!)? status) -> (Tensor, Tensor)",
-      &pla_ops::qk_rotary);
+      "apply_rotary(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, float factor, bool interleaved, Tensor(a!)? out_q=None, "
+      "Tensor(b!)? out_k=None) -> (Tensor, Tensor)",
+      &pla_ops::apply_rotary);
   m.def(
-      "paged_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float? scale, "
-      "Tensor(a!)? out, bool return_lse, Tensor(b!)? status) -> (Tensor, Tensor)",
+      "qk_norm_rotary(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor positions, Tensor inv_freq, float eps, float factor, "
+      "bool interleaved, bool unit_offset, Tensor(a!)? out_q=None, Tensor(b!)? out_k=None) -> (Tensor, Tensor)",
+      &pla_ops::qk_norm_rotary);
+  m.def(
+      "qk_norm_rotary_cache(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor positions, Tensor inv_freq, "
+      "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slot_mapping, float eps, float factor, bool interleaved, bool unit_offset, "
+      "Tensor(c!)? out_q=None, Tensor(d!)? status=None) -> Tensor",
+      &pla_ops::qk_norm_rotary_cache);
+  m.def(
+      "paged_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float? scale, bool return_lse, "
+      "Tensor(a!)? out=None, Tensor(b!)? status=None) -> (Tensor, Tensor)",
       &pla_ops::paged_attention_decode);
 }

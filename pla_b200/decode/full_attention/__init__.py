@@ -21,9 +21,12 @@ import torch
 
 from ..._ops import ops
 
-# the overloads themselves: half a microsecond less per call than looking them up through their packets
+# The overloads themselves: half a microsecond less per call than looking them up through their packets. Arguments that are
+# not given are left out of the calls below for the same reason.
 _block_tables = ops.build_block_tables.default
-_rotary = ops.qk_rotary.default
+_rotary = ops.apply_rotary.default
+_norm_rotary = ops.qk_norm_rotary.default
+_norm_rotary_cache = ops.qk_norm_rotary_cache.default
 _paged_decode = ops.paged_attention_decode.default
 
 __all__ = [
@@ -68,8 +71,12 @@ def build_block_tables(
     ``status`` (int32[1]) gets 32 when the list ran out and 64 when a row has too few columns (the tokens without a page
     have slot -1), 1 for negative lengths and for offsets past ``num_tokens``.
     """
-    slots, positions, seq_lens, free_next = _block_tables(
-        block_table, context_lens, query_start_loc, free_blocks, block_size, num_tokens, free_start, status)
+    if status is None:
+        slots, positions, seq_lens, free_next = _block_tables(
+            block_table, context_lens, query_start_loc, free_blocks, block_size, num_tokens, free_start)
+    else:
+        slots, positions, seq_lens, free_next = _block_tables(
+            block_table, context_lens, query_start_loc, free_blocks, block_size, num_tokens, free_start, status)
     return BlockPlan(block_table, slots, positions, seq_lens, free_next)
 
 
@@ -148,7 +155,9 @@ def apply_rotary(
     """Rotates the first ``2 * len(inv_freq)`` channels of every head of ``q`` ``[tokens, heads, dim]`` and ``k``
     by ``positions[t] * inv_freq`` and multiplies them by ``factor``; the other channels are copied. Pairs are ``(i, i + R/2)``, or
     ``(2i, 2i + 1)`` with ``interleaved``. ``out_q=q`` / ``out_k=k`` rotate in place."""
-    return _rotary(q, k, None, None, None, positions, inv_freq, None, None, None, 0.0, factor, interleaved, False, out_q, out_k, None)
+    if out_q is None and out_k is None:
+        return _rotary(q, k, positions, inv_freq, factor, interleaved)
+    return _rotary(q, k, positions, inv_freq, factor, interleaved, out_q, out_k)
 
 
 def qk_norm_rotary(
@@ -168,8 +177,9 @@ def qk_norm_rotary(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """RMS norm of every head of ``q`` and ``k`` (``x * rsqrt(mean(x^2) + eps) * weight``, ``1 + weight`` with ``unit_offset``; a
     ``None`` weight leaves that side as it is), then the rotation of :func:`apply_rotary`, in one pass."""
-    return _rotary(q, k, None, q_weight, k_weight, positions, inv_freq, None, None, None, eps, factor, interleaved, unit_offset, out_q, out_k,
-                   None)
+    if out_q is None and out_k is None:
+        return _norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, eps, factor, interleaved, unit_offset)
+    return _norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, eps, factor, interleaved, unit_offset, out_q, out_k)
 
 
 def qk_norm_rotary_cache(
@@ -194,8 +204,11 @@ def qk_norm_rotary_cache(
     """:func:`qk_norm_rotary` whose keys go to ``k_cache[slot // block_size, slot % block_size]`` (``[blocks, block_size, kv heads, dim]``
     with any strides) and whose values are copied to ``v_cache`` likewise; returns the queries. A negative slot stores
     nothing; a slot outside the pool stores nothing and sets 8 in ``status``. The slots of a call must differ."""
-    return _rotary(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
-                   unit_offset, out_q, None, status)[0]
+    if out_q is None and status is None:
+        return _norm_rotary_cache(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
+                                  unit_offset)
+    return _norm_rotary_cache(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
+                              unit_offset, out_q, status)
 
 
 def paged_attention_decode(
@@ -217,5 +230,8 @@ def paged_attention_decode(
 
     ``status`` (int32[1]) gets 1 for a length that is negative or past the table's row, 8 for a page outside the pool (its
     tokens are left out)."""
-    o, lse = _paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, return_lse, status)
+    if out is None and status is None:
+        o, lse = _paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, return_lse)
+    else:
+        o, lse = _paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, return_lse, out, status)
     return (o, lse) if return_lse else o
