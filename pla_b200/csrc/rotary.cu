@@ -11,8 +11,8 @@
 // to a fraction of a turn in 64 bits (in 32 bits whole radians are lost at positions of a million), take sine and cosine in 32 bits and
 // share them through shared memory. Warps are persistent and bring the next rows, of the next token as well, through a ring of
 // 16-byte asynchronous copies into cells that only the copying lane reads.
-// On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 109 us, 6.1 TB/s; rotation alone of 32,761
-// tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 123 us, 5.5 TB/s; 1,999 tokens with the norm (41 MB) 13 us; one token 3 us. At 2.6
+// On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 112 us, 6.0 TB/s; rotation alone of 32,761
+// tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 119 us, 5.6 TB/s; 1,999 tokens with the norm (41 MB) 12 us; one token 3 us. At 2.6
 // instructions per cycle and SM the arithmetic alone takes about 75 us of these; a seventh fewer instructions did not shorten the large
 // calls, so what is left is how well reads and writes overlap. Measured and not kept: two channels per instruction (fma.f32x2; the register pairs cost more moves than it saves, 61 -> 83 million instructions for
 // the interleaved case), three CTAs per SM (80 registers spill, 167 us), 64-bit floating-point angles (the wrapped integers are exact and
