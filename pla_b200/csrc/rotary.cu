@@ -5,18 +5,18 @@
 // (heads) of one token, or a share of them when there are few tokens; a row belongs to a group of 4, 8 or 16 lanes, and a lane holds
 // eight channels of the row's first half and eight of its second. With y = inv x w (inv from the group's sum of squares) and the
 // pair's other channel x', the rotated channel is inv (x A + x' B), A = w cos and B = -+ w' sin: weights, sines and cosines are folded
-// once per token and side, and a channel costs two multiply-adds. x' is the lane's other half
-// (whole head rotated), the same lane's neighbour (interleaved), comes from the lane R/16 away as the raw 16-bit row (up to half the
-// head rotated), or from memory again where the rotated part does not fit these. Angles: the warp's lanes reduce position * frequency
-// to a fraction of a turn in 64 bits (in 32 bits whole radians are lost at positions of a million), take sine and cosine in 32 bits and
-// share them through shared memory. Warps are persistent and bring the next rows, of the next token as well, through a ring of
-// 16-byte asynchronous copies into cells that only the copying lane reads.
+// once per token and side, and a channel costs two multiply-adds. x' is the lane's other half (whole head rotated), the same lane's
+// neighbour (interleaved), comes from the lane R/16 away as the raw 16-bit row (up to half the head rotated), or from that lane's cell in
+// shared memory (other sizes of the rotated part). Angles: the warp's lanes reduce position * frequency to a fraction of a turn in 64 bits
+// (in 32 bits whole radians are lost at positions of a million), take sine and cosine in 32 bits and share them through shared
+// memory. Warps are persistent and bring the next rows, of the next token as well, through a ring of 16-byte asynchronous copies,
+// each lane into cells of its own.
 // On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 112 us, 6.0 TB/s; rotation alone of 32,761
 // tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 119 us, 5.6 TB/s; 1,999 tokens with the norm (41 MB) 12 us; one token 3 us. At 2.6
 // instructions per cycle and SM the arithmetic alone takes about 75 us of these; a seventh fewer instructions did not shorten the large
-// calls, so what is left is how well reads and writes overlap. Measured and not kept: two channels per instruction (fma.f32x2; the register pairs cost more moves than it saves, 61 -> 83 million instructions for
-// the interleaved case), three CTAs per SM (80 registers spill, 167 us), 64-bit floating-point angles (the wrapped integers are exact and
-// a few percent faster).
+// calls, so what is left is how well reads and writes overlap. Measured and not kept: two channels per instruction (fma.f32x2: the
+// register pairs cost more moves than it saves, 61 -> 83 million instructions for the interleaved case), three CTAs per SM (80 registers
+// spill, 167 us), angles in 64-bit floating point (the wrapped integers are exact and a few percent faster).
 #include "common.cuh"
 #include "../../include/pla_b200_attention.h"
 
