@@ -25,8 +25,9 @@
 // between the first and the last CTA to finish (SMs get unequal shares of the bandwidth), and 4 us for the join. Handing out the last
 // eighth or quarter of the units from a counter evened the CTAs out, but the additional parts cost the join more (91 -> 109 us for 128K);
 // shares by tiles and item ends instead of units gained 5 % for 200 requests up to 300 tokens and cost small calls 0.7 us.
-// Scores, sums and outputs are 32-bit; the weights p are rounded to the activations' type for the product with V (relative 2^-8
-// or 2^-11, the same size as the output's own rounding), the sum of the weights is of the unrounded ones.
+// Scores, sums and outputs are 32-bit. The matrix unit takes weights p of the activations' type, so each goes in as two numbers, its rounding and
+// what the rounding left, and V is multiplied by both: relative 2^-16 (bf16) or 2^-22 (fp16), far below the output's own rounding.
+// fp16 loses small numbers, so its weights are 2^7 (SHIFT) times as large: what is lost of one is at most 2^-32 of the largest.
 #include <cuda.h>
 
 #include <type_traits>
@@ -43,7 +44,12 @@ constexpr int TILE = 16;              // tokens per warp and step
 constexpr int UNIT = TILE * WARPS;    // tokens per CTA and step
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float SLACK = 8.0f;         // the running maximum may lag this far (log2) behind: p stays below 2^8, fewer rescalings
+constexpr float SLACK = 8.0f;         // the running maximum may lag this far (log2) behind: fewer rescalings
+// The maximum that a warp keeps is this far (log2) below the scores': weights reach 2^(SHIFT + SLACK), 2^15 of the 65,504 that fp16 holds.
+template <typename act_t>
+constexpr float SHIFT = 0.0f;
+template <>
+constexpr float SHIFT<__half> = 7.0f;
 
 // Ring depth, and CTAs per SM that its shared memory leaves room for (of 227 KB): 192 KB of rows in flight per SM.
 template <int D>
@@ -85,6 +91,17 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+template <typename act_t>
+__device__ __forceinline__ float2 widen(uint32_t two);
+template <>
+__device__ __forceinline__ float2 widen<__nv_bfloat16>(uint32_t two) {
+  return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 widen<__half>(uint32_t two) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&two));
 }
 
 template <typename act_t>
@@ -560,7 +577,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma<act_t>(s[n][kk & 1], a, qf[kk][n]);
       }
-      uint32_t pf[NT][2];
+      uint32_t pf[NT][2], rest[NT][2];       // weights, and what their rounding left
       float next[NT][2];
       bool grow = false;
 #pragma unroll
@@ -578,8 +595,8 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           float x = fmaxf(c[e], c[e + 2]);
 #pragma unroll
           for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
-          next[n][e] = x;
-          grow |= x > m[n][e] + SLACK;
+          next[n][e] = x - SHIFT<act_t>;
+          grow |= next[n][e] > m[n][e] + SLACK;
         }
       }
       if (__any_sync(0xffffffffu, grow)) {
@@ -611,8 +628,13 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
           c[e] = fast_exp2(c[e] - (top == -INFINITY ? 0.0f : top));
           l[n][e & 1] += c[e];
         }
-        pf[n][0] = transpose8x8(pack2<act_t>(c[0], c[1]));
-        pf[n][1] = transpose8x8(pack2<act_t>(c[2], c[3]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t two = pack2<act_t>(c[2 * h], c[2 * h + 1]);
+          const float2 kept = widen<act_t>(two);
+          pf[n][h] = transpose8x8(two);
+          rest[n][h] = transpose8x8(pack2<act_t>(c[2 * h] - kept.x, c[2 * h + 1] - kept.y));
+        }
       }
       const uint32_t va = v_rows + ((lane & 7) + (lane >> 4) * 8) * 128;
 #pragma unroll
@@ -620,7 +642,10 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
         uint32_t a[4];
         ldmatrix4_trans(a, va + (kk / 4) * S::BOX + ((((kk % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma<act_t>(o[kk][n], a, pf[n]);
+        for (int n = 0; n < NT; ++n) {
+          mma<act_t>(o[kk][n], a, pf[n]);
+          mma<act_t>(o[kk][n], a, rest[n]);
+        }
       }
     }
     __syncwarp();

@@ -531,6 +531,37 @@ def test_attention_peaked_and_extreme_scores(native_built):
         assert_attention(out, lse, q, kc, vc, table, lens, scale)
 
 
+def assert_attention_kept(got, lse, q, kc, vc, table, lens, scale=None):
+    """``assert_attention`` with the weights of the softmax held in more bits than one number of the activations' type: as two of them, each
+    is within half(t)^2 of itself; an fp16 weight also within 2^-32 of the largest one, 2^-25 (half of fp16's smallest step) with the
+    weights 2^7 times as large. The rest of the bound is the same."""
+    out, want_lse, spread, reach = ofa.paged_attention(q, kc.cpu(), vc.cpu(), table, lens, scale)
+    D, n = q.shape[-1], torch.tensor([max(int(x), 0) for x in lens], dtype=torch.float64)[:, None]
+    e, sums = D * 2.0 ** -24 * reach, (n + 64) * 2.0 ** -24
+    lost = 0.0
+    if q.dtype == torch.float16:
+        bs, heads = kc.shape[1], q.shape[1] // kc.shape[2]
+        lost = torch.zeros_like(out)
+        for b, length in enumerate(lens):
+            t = torch.arange(max(int(length), 0))
+            v = vc.cpu()[table[b, t // bs].long(), t % bs].double().abs().sum(0)          # [kv heads, channels]
+            lost[b] = 2.0 ** -32 * v.repeat_interleave(heads, 0)                           # the largest weight is at most 1
+    assert_within(got, out, (half(q.dtype) ** 2 + 2 * e + 2 * sums + 2.0 ** -20)[..., None] * spread + lost)
+    if lse is not None:
+        assert_attention(got, lse, q, kc, vc, table, lens, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lens,hq,hk,D,bs,layout", [(EDGES, 16, 2, 256, 16, "separate"), (EDGES, 5, 1, 96, 7, "separate"), (EDGES, 33, 1, 128, 16, "packed"),
+                                                    (EDGES, 12, 3, 64, 1, "heads"), ([777], 16, 2, 128, 16, "separate"), ([0, 70, 513], 34, 2, 192, 32, "packed")])
+def test_attention_keeps_the_weights(native_built, lens, hq, hk, D, bs, layout, dtype):
+    """The output is the 32-bit value, rounded once: the weights' own rounding does not show."""
+    q, kc, vc, table = paged_inputs(hq + D, lens, hq, hk, D, bs, DT[dtype], layout, extra_columns=0)
+    out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), return_lse=True)
+    assert_attention_kept(out, lse, q, kc, vc, table, lens)
+
+
 @pytest.mark.gpu
 def test_attention_views_and_streams(native_built):
     """q as a slice of a wider row and with heads outermost, a table that is a slice of a wider one, another stream, two calls at
