@@ -563,6 +563,25 @@ def test_attention_keeps_the_weights(native_built, lens, hq, hk, D, bs, layout, 
 
 
 @pytest.mark.gpu
+def test_attention_fp16_tail_behind_one_token(native_built):
+    """One token 25.1 powers of two above 2^16 - 1 others: fp16 has no number that small beside 1, but the sum counts them. All values are 1, so
+    the output is exactly 1. There is one request per CTA (three of 64 channels per SM), so that one warp owns the large weight and 2^14 of the
+    small ones, 2^-11.1 in all: without them the output is a step below 1. Bound: the 2^10 sums of 16 tokens on the matrix unit are off
+    by at most 2^-23 each, 2^-13; the 2^11 additions of the lane that holds the large weight by at most one small weight each, 2^-14.1;
+    the weights in fp16 by 2^-32 each, 2^-18: together below 2^-12, half the step below 1."""
+    B, D, bs, n = 3 * torch.cuda.get_device_properties(0).multi_processor_count, 64, 64, 1 << 16
+    kc = torch.full((2, bs, 1, D), -1.0, dtype=torch.float16, device="cuda")
+    kc[0, 0] = 0
+    vc = torch.ones_like(kc)
+    table = torch.ones(1, n // bs, dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    out, lse = fa().paged_attention_decode(torch.ones(B, 1, D, dtype=torch.float16, device="cuda"), kc, vc, table.expand(B, -1), i32([n] * B),
+                                           scale=25.1 * math.log(2) / D, return_lse=True)
+    assert torch.all(out == 1)
+    assert (lse.double() - math.log1p((n - 1) * 2.0 ** -25.1)).abs().max().item() <= 2.0 ** -13
+
+
+@pytest.mark.gpu
 def test_attention_views_and_streams(native_built):
     """q as a slice of a wider row and with heads outermost, a table that is a slice of a wider one, another stream, two calls at
     once: the same results."""
