@@ -268,6 +268,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
     }
   };
   Place at;
+  int item_units = 0;                      // TEAMED: of the cluster's item
   int64_t total = 0, workers = 1, begin, end;
   if constexpr (TEAMED) {
     const int item = blockIdx.x / TEAM, rank = blockIdx.x % TEAM;
@@ -276,8 +277,9 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
     at.chunk = item - at.b * items - at.head * plan.chunks;
     at.len = length_of(p, at.b, bad);
     at.units = (at.len + UNIT - 1) / UNIT;
-    begin = static_cast<int64_t>(at.units) * rank / TEAM;
-    end = static_cast<int64_t>(at.units) * (rank + 1) / TEAM;
+    item_units = at.units;
+    begin = item_units * rank / TEAM;
+    end = item_units * (rank + 1) / TEAM;
     at.unit = static_cast<int>(begin);
     if (tid < 8 * NT) s_part_m[tid] = -INFINITY;
     __syncthreads();
@@ -473,6 +475,7 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
   };
 
   // Joins the four warps' parts of the item that ends here (or leaves the range) and stores them: as output, or as a part.
+  // A NaN score leaves the maximum where it is and makes the sum NaN: what has no weight is known by its sum, not by its maximum.
   auto flush = [&](const Place& x, bool whole, int slot) {
     const int head = x.head * plan.group + x.chunk * 8 * NT, heads = min(8 * NT, plan.group - x.chunk * 8 * NT);
     const int64_t first_row = static_cast<int64_t>(x.b) * p.Hq + head, first_part = static_cast<int64_t>(slot) * 8 * NT;
@@ -498,9 +501,10 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
         float top = -INFINITY, weight = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][h]);
+        const float base = top == -INFINITY ? 0.0f : top;       // exp2(-inf - base) = 0
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) weight += s_m[w][h] == -INFINITY ? 0.0f : s_l[w][h] * fast_exp2(s_m[w][h] - top);
-        down[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - top);
+        for (int w = 0; w < WARPS; ++w) weight += s_l[w][h] * fast_exp2(s_m[w][h] - base);
+        down[i] = fast_exp2(m[n][i] - base);
         if (whole) down[i] = weight == 0.0f ? 0.0f : down[i] / weight;
         if (warp == 0 && lane < 4 && h < heads) {
           if (!whole) {
@@ -689,10 +693,11 @@ paged_decode_kernel(const pla_b200_paged_decode_args p, const Plan plan, const _
       for (int r = 0; r < TEAM; ++r) part_m[r] = team_load(team_addr(smem_addr(&s_part_m[h]), r));
 #pragma unroll
       for (int r = 0; r < TEAM; ++r) top = fmaxf(top, part_m[r]);
+      const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
       for (int r = 0; r < TEAM; ++r) {
-        if (part_m[r] == -INFINITY) continue;                                     // nothing was stored there
-        const float f = fast_exp2(part_m[r] - top);
+        if (item_units * r / TEAM == item_units * (r + 1) / TEAM) continue;       // had no units and stored nothing
+        const float f = fast_exp2(part_m[r] - base);
         const float4 x = team_load4(team_addr(ring + (h * D + d) * 4, r));
         weight += team_load(team_addr(smem_addr(&s_part_l[h]), r)) * f;
         sum.x += x.x * f, sum.y += x.y * f, sum.z += x.z * f, sum.w += x.w * f;

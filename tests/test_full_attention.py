@@ -582,6 +582,33 @@ def test_attention_fp16_tail_behind_one_token(native_built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("wide", [False, True], ids=["clusters", "two-kernels"])
+@pytest.mark.parametrize("hq,hk,D,bs", [(4, 2, 64, 16), (3, 1, 256, 16), (18, 2, 128, 7), (6, 1, 96, 1)])
+@pytest.mark.parametrize("where", ["query", "newest key", "first key", "all keys", "value"])
+def test_attention_nan_stays(native_built, where, hq, hk, D, bs, wide, dtype):
+    """A NaN reaches every output and sum of the softmax that it is part of, whichever way the call takes and whatever the CTA or warp that
+    holds it has besides; rows of length 0 stay zeros. Everything else keeps its bound."""
+    lens = [1, 64, 65, 0, 300, 16]
+    q, kc, vc, table = paged_inputs(D + hq, lens, hq, hk, D, bs, DT[dtype], extra_columns=20000 // bs if wide else 0)
+    if where == "query":
+        q[:, 1, D // 2] = float("nan")
+    for b, n in enumerate(lens):
+        for t in {"newest key": [n - 1], "first key": [0], "all keys": range(n), "value": [n // 2]}.get(where, []):
+            if n:
+                (vc if where == "value" else kc)[table[b, t // bs].item(), t % bs, hk - 1, 3] = float("nan")
+    out, lse = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens), return_lse=True)
+    want, want_lse, spread, reach = ofa.paged_attention(q, kc.cpu(), vc.cpu(), table, lens)
+    assert torch.equal(out.isnan().cpu(), want.isnan()) and torch.equal(lse.isnan().cpu(), want_lse.isnan())
+    assert want.isnan().any() and not want.isnan().all()
+    e, sums = D * 2.0 ** -24 * reach.nan_to_num(0.0), 400 * 2.0 ** -24
+    assert_within(out.nan_to_num(0.0), want.nan_to_num(0.0), (half(q.dtype) + 2 * e + 2 * sums + 2.0 ** -20)[..., None] * spread.nan_to_num(0.0))
+    live = torch.isfinite(want_lse)
+    assert torch.equal(lse.cpu()[3], torch.full((hq,), -math.inf))
+    assert ((lse.cpu().double() - want_lse).abs() - e - sums - 2.0 ** -22 * (1 + want_lse.abs()))[live].le(0).all()
+
+
+@pytest.mark.gpu
 def test_attention_views_and_streams(native_built):
     """q as a slice of a wider row and with heads outermost, a table that is a slice of a wider one, another stream, two calls at
     once: the same results."""
