@@ -13,11 +13,13 @@ def block_tables(block_table, context_lens, offsets, free, block_size, num_token
     columns = len(table[0]) if table else 0
     slots, positions, lens, status, at = [-1] * num_tokens, [0] * num_tokens, [], 0, start
     for n, (c, lo, hi) in enumerate(zip(context_lens, offsets, offsets[1:])):
-        m = hi - lo
-        if c < 0 or m < 0:
+        if c < 0 or hi < lo or c + hi - lo >= 1 << 31:
             status |= 1
             lens.append(max(c, 0))
             continue
+        if hi > num_tokens:                       # what has no row is left out
+            status |= 1
+        m = min(hi, num_tokens) - min(lo, num_tokens)
         lens.append(c + m)
         held, wanted = -(-c // block_size), -(-(c + m) // block_size)
         if wanted > columns:

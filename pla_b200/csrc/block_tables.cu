@@ -54,10 +54,12 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
         if (first_cta) p.seq_lens[n] = max(ctx[i], 0);
         s_ctx[tid * PER + i] = -1;
       } else {
-        const int all = pages(ctx[i] + static_cast<int>(m));
+        // tokens past the caller's rows have no thread that could enter a page for them: they are left out of everything
+        const int len = ctx[i] + min(off[i + 1], p.tokens) - min(off[i], p.tokens), all = pages(len);
         need[i] = max(min(all, p.columns) - pages(ctx[i]), 0);
+        if (off[i + 1] > p.tokens) bad |= PLA_B200_DEV_BAD_INTERVAL;
         if (all > p.columns) bad |= PLA_B200_DEV_TABLE_FULL;
-        if (first_cta) p.seq_lens[n] = static_cast<int32_t>(ctx[i] + m);
+        if (first_cta) p.seq_lens[n] = len;
         s_ctx[tid * PER + i] = ctx[i];
       }
       s_off[tid * PER + i] = off[i];
@@ -112,7 +114,6 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
       }
     }
     running += total;
-    if (first_cta && n0 + cnt == p.N && hi > p.tokens) bad |= PLA_B200_DEV_BAD_INTERVAL;    // rows that the caller has no room for
     if (!first_cta && lo > t0 + TPB - 1) break;     // the tile's tokens lie behind us
     __syncthreads();                       // the next chunk overwrites the shared arrays
   }

@@ -199,6 +199,21 @@ def test_tables_edges(native_built):
 
 
 @pytest.mark.gpu
+def test_tables_leave_out_tokens_without_a_row(native_built):
+    """Offsets past the token rows: pages, table entries, lengths and the list's next entry agree on the tokens that have a row."""
+    want = tables_case([0, 0], [2, 7], 4, tokens=3)
+    assert want[5] == 1 and want[3] == [2, 1] and want[4] == 2
+    want = tables_case([6, 3, 8, 0], [5, 9, 1, 40], 4, tokens=8)                  # ends inside a request that holds pages
+    assert want[5] == 1 and want[3] == [11, 6, 8, 0]
+    want = tables_case([4] * 3, [4] * 3, 4, tokens=0)
+    assert want[5] == 1 and want[3] == [4] * 3 and want[4] == 0
+    want = tables_case([i % 9 for i in range(1500)], [3] * 1500, 2, tokens=2000)  # in the middle of the first scan of two
+    assert want[5] == 1 and want[3][667:] == [i % 9 for i in range(667, 1500)]
+    want = tables_case([5, 2 ** 31 - 3], [1, 3], 1 << 20, columns=4)              # a length past 32 bits
+    assert want[5] == 1 and want[3] == [6, 2 ** 31 - 3] and want[1][1:] == [-1] * 3
+
+
+@pytest.mark.gpu
 def test_tables_with_many_requests_and_streams(native_built):
     """More requests than one scan holds, several tiles of tokens; the same on another stream and replayed from a graph with other
     lengths in the same tensors."""
