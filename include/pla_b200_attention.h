@@ -30,10 +30,11 @@ typedef struct pla_b200_page_strides {
  *   block_table[n, held + j] = free_blocks[start + (sum of need before n) + j]
  * Token t of request n sits at position p = c + t - query_start_loc[n] and in slot
  * block_table[n, p / block_size] * block_size + p % block_size. Other entries of the table keep their values. Tokens at or past
- * query_start_loc[N], tokens without a page and tokens of a request with bad metadata (c < 0, m < 0 or c + m past 32 bits:
- * it takes no pages, seq_lens[n] = max(c, 0), PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last
- * kind. A page past the end of the free list becomes -1. `tokens` has to cover query_start_loc[N]; where it does not, the new tokens
- * past it are left out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs (block_table is both).
+ * query_start_loc[N], tokens without a page and tokens of a request with bad metadata (c < 0, m < 0, c + m past 32 bits, or an
+ * offset query_start_loc[n] that is negative or below an earlier one: it takes no pages, seq_lens[n] = max(c, 0),
+ * PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last kind. A page past the end of the free list becomes -1. `tokens` has to cover query_start_loc[N], which has to be the largest offset; new tokens past
+ * either are left out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs
+ * (block_table is both).
  * ======================================================================== */
 typedef struct pla_b200_block_tables_args {
   int32_t* block_table;           /* [N, columns], pages of the context already in place */

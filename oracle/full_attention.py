@@ -10,16 +10,16 @@ import torch
 def block_tables(block_table, context_lens, offsets, free, block_size, num_tokens, start=0):
     """Lists in, ``(table, slots, positions, seq_lens, free_next, status)`` out; status bits as the kernel reports them."""
     table = [list(row) for row in block_table]
-    columns = len(table[0]) if table else 0
+    columns, rows = len(table[0]) if table else 0, min(max(offsets[-1], 0), num_tokens)
     slots, positions, lens, status, at = [-1] * num_tokens, [0] * num_tokens, [], 0, start
     for n, (c, lo, hi) in enumerate(zip(context_lens, offsets, offsets[1:])):
-        if c < 0 or hi < lo or c + hi - lo >= 1 << 31:
+        if c < 0 or hi < lo or lo < max([0] + offsets[:n]) or c + hi - lo >= 1 << 31:
             status |= 1
             lens.append(max(c, 0))
             continue
-        if hi > num_tokens:                       # what has no row is left out
+        if hi > rows:                             # what has no row is left out
             status |= 1
-        m = min(hi, num_tokens) - min(lo, num_tokens)
+        m = min(hi, rows) - min(lo, rows)
         lens.append(c + m)
         held, wanted = -(-c // block_size), -(-(c + m) // block_size)
         if wanted > columns:
@@ -31,7 +31,7 @@ def block_tables(block_table, context_lens, offsets, free, block_size, num_token
                 table[n][col] = -1
                 status |= 32
             at += 1
-        for t in range(lo, min(hi, num_tokens)):
+        for t in range(lo, min(hi, rows)):
             p = c + t - lo
             positions[t] = p
             if p // block_size < columns and table[n][p // block_size] >= 0:

@@ -19,7 +19,7 @@ constexpr int CHUNK = TPB * PER;
 
 __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_tables_args p, const Divisor page_size) {
   auto pages = [&](int n) { return n > 0 ? page_size.quotient(n - 1) + 1 : 0; };      // that n tokens fill
-  __shared__ int32_t s_off[CHUNK + 1];     // offsets of the chunk's requests
+  __shared__ int32_t s_off[CHUNK + 1];     // offsets of the chunk's requests, none below an earlier one
   __shared__ int32_t s_ctx[CHUNK];         // tokens in the cache; -1: bad metadata, no slots
   __shared__ int64_t s_base[CHUNK];        // first entry of the free list that the request takes
   __shared__ int64_t s_warp[TPB / 32];
@@ -28,9 +28,10 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
   const int t = t0 + tid;
   const bool first_cta = blockIdx.x == 0;  // writes what there is per request
   const int64_t start = p.free_start != nullptr ? max(*p.free_start, 0) : 0;
+  const int rows = min(max(p.query_start_loc[p.N], 0), p.tokens);       // the others are padding
   int64_t running = start;
   int64_t slot = -1, pos = 0;
-  int32_t bad = 0;
+  int32_t bad = 0, highest = 0;            // of the offsets so far
   for (int n0 = 0; n0 < p.N; n0 += CHUNK) {
     const int cnt = min(CHUNK, p.N - n0);
     int32_t off[PER + 1], ctx[PER];
@@ -43,27 +44,46 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
       ctx[i] = n < p.N ? p.context_lens[n] : 0;
     }
     off[PER] = n0 + tid * PER + PER <= p.N ? p.query_start_loc[n0 + tid * PER + PER] : 0;
+    // Offsets that are negative or fall (bad metadata): a request that begins below an earlier offset would share its tokens with another
+    // one, and only one of them could enter pages there. It gets none; the search goes by the largest offset up to each request.
+    int top[PER + 1];
+    bool falls = false;
+#pragma unroll
+    for (int i = 0; i <= PER; ++i) {
+      top[i] = off[i];
+      if (n0 + tid * PER + i <= p.N) falls |= off[i] < (i > 0 ? off[i - 1] : highest);
+    }
+    if (__syncthreads_or(falls)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) s_off[tid * PER + i] = off[i];
+      __syncthreads();
+      int most = highest;
+      for (int j = 0; j < tid * PER; ++j) most = max(most, s_off[j]);
+#pragma unroll
+      for (int i = 0; i <= PER; ++i) top[i] = most = max(most, off[i]);
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int n = n0 + tid * PER + i;
       need[i] = 0;
       if (n >= p.N) continue;
       const int64_t m = static_cast<int64_t>(off[i + 1]) - off[i];
-      if (m < 0 || ctx[i] < 0 || ctx[i] + m > INT32_MAX) {
+      if (m < 0 || off[i] < top[i] || ctx[i] < 0 || ctx[i] + m > INT32_MAX) {
         bad |= PLA_B200_DEV_BAD_INTERVAL;
         if (first_cta) p.seq_lens[n] = max(ctx[i], 0);
         s_ctx[tid * PER + i] = -1;
       } else {
-        // tokens past the caller's rows have no thread that could enter a page for them: they are left out of everything
-        const int len = ctx[i] + min(off[i + 1], p.tokens) - min(off[i], p.tokens), all = pages(len);
+        // tokens without a row have no thread that could enter a page for them: they are left out of everything
+        const int len = ctx[i] + min(off[i + 1], rows) - min(off[i], rows), all = pages(len);
         need[i] = max(min(all, p.columns) - pages(ctx[i]), 0);
-        if (off[i + 1] > p.tokens) bad |= PLA_B200_DEV_BAD_INTERVAL;
+        if (off[i + 1] > rows) bad |= PLA_B200_DEV_BAD_INTERVAL;
         if (all > p.columns) bad |= PLA_B200_DEV_TABLE_FULL;
         if (first_cta) p.seq_lens[n] = len;
         s_ctx[tid * PER + i] = ctx[i];
       }
-      s_off[tid * PER + i] = off[i];
-      if (n + 1 == p.N || tid * PER + i + 1 == CHUNK) s_off[tid * PER + i + 1] = off[i + 1];
+      s_off[tid * PER + i] = top[i];
+      if (n + 1 == p.N || tid * PER + i + 1 == CHUNK) s_off[tid * PER + i + 1] = top[i + 1];
       mine += need[i];
     }
     int64_t upto = mine;                   // inclusive scan over the block
@@ -89,7 +109,7 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
     }
     __syncthreads();
     const int32_t lo = s_off[0], hi = s_off[cnt];
-    if (t < p.tokens && t >= lo && t < hi) {
+    if (t < rows && t >= lo && t < hi) {
       int a = 0, b = cnt;                  // s_off[a] <= t < s_off[b]
       while (b - a > 1) {
         const int mid = (a + b) >> 1;
@@ -114,6 +134,7 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
       }
     }
     running += total;
+    highest = hi;
     if (!first_cta && lo > t0 + TPB - 1) break;     // the tile's tokens lie behind us
     __syncthreads();                       // the next chunk overwrites the shared arrays
   }

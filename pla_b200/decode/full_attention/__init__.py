@@ -69,7 +69,7 @@ def build_block_tables(
     -1 and position 0. Pass ``free_next`` as the next step's ``free_start`` to go on in the same list.
 
     ``status`` (int32[1]) gets 32 when the list ran out and 64 when a row has too few columns (the tokens without a page
-    have slot -1), 1 for negative lengths and for offsets past ``num_tokens`` (new tokens past it are left out: no page, not in
+    have slot -1), 1 for negative lengths, offsets that are negative or fall (such a request gets nothing) and for offsets past ``num_tokens`` (new tokens past it are left out: no page, not in
     ``seq_lens``).
     """
     if status is None:

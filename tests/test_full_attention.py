@@ -125,9 +125,9 @@ def test_abi_entries_are_exported_and_refuse_bad_arguments(native_built):
 
 
 # ------------------------------------------------------------------------------------------------ block tables
-def tables_case(context, new, block_size, columns=None, tokens=None, free=None, start=None, pad=0):
+def tables_case(context, new, block_size, columns=None, tokens=None, free=None, start=None, pad=0, first=0):
     """Runs op and oracle on one batch and compares everything, bit for bit."""
-    offsets = [0]
+    offsets = [first]
     for m in new:
         offsets.append(offsets[-1] + m)
     held = [max(0, -(-c // block_size)) for c in context]
@@ -135,7 +135,7 @@ def tables_case(context, new, block_size, columns=None, tokens=None, free=None, 
     if columns is None:
         columns = max([-(-(c + m) // block_size) for c, m in zip(context, new)] + [1]) + 1
     g = torch.Generator().manual_seed(len(context) * 31 + block_size)
-    ids = torch.randperm(sum(held) + need + 5, generator=g).tolist()
+    ids = torch.randperm(sum(held) + max(need, free or 0, 0) + 5, generator=g).tolist()
     rows, at = [], 0
     for h in held:
         h = min(h, columns)
@@ -211,6 +211,21 @@ def test_tables_leave_out_tokens_without_a_row(native_built):
     assert want[5] == 1 and want[3][667:] == [i % 9 for i in range(667, 1500)]
     want = tables_case([5, 2 ** 31 - 3], [1, 3], 1 << 20, columns=4)              # a length past 32 bits
     assert want[5] == 1 and want[3] == [6, 2 ** 31 - 3] and want[1][1:] == [-1] * 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("context,new,first,tokens", [
+    ([0, 0, 0], [4, -2, 4], 0, 6), ([1] * 5, [10, -8, 1, 1, 8], 0, 12), ([3, 2], [5, 1], -3, 4), ([0] * 4, [3, -5, 9, 2], 0, 9),
+    ([2] * 3, [1, 1, 1], 5, 10), ([0, 0], [-2, 6], 0, 8), ([0, 0], [4, -2], 0, 4), ([0, 0], [4, -6], 0, 4), ([i % 7 for i in range(2500)], [1] * 700 + [-300] + [2] * 1799, 0, 4100),
+    ([i % 7 for i in range(2500)], [1] * 1023 + [-900, 2] + [1] * 1475, 0, 1700), ([1] * 1500, [3] * 1500, -2000, 2600)],
+    ids=["falls", "long", "negative", "below-0", "late", "at-once", "end-falls", "end-below-0", "in-a-scan", "between-scans", "far-below"])
+def test_tables_offsets_that_fall(native_built, context, new, first, tokens):
+    """Requests that begin below an earlier offset, or below 0, get nothing; table, slots, lengths and the list agree on the others."""
+    for block_size in (1, 3, 16):
+        want = tables_case(context, new, block_size, tokens=tokens, first=first, columns=16, free=5200)
+        assert want[5] == (0 if first > 0 else 1)
+        taken = [x for x in want[1] if x >= 0]
+        assert len(set(taken)) == len(taken)
 
 
 @pytest.mark.gpu
