@@ -158,7 +158,7 @@ extern "C" int pla_b200_block_tables(const pla_b200_block_tables_args* args, voi
   PLA_REQUIRE(a.N >= 0 && a.tokens >= 0 && a.columns >= 0 && a.free_count >= 0 && a.block_size > 0, PLA_B200_E_INVALID,
               "block tables need N, tokens, columns, free_count >= 0 and block_size > 0");
   PLA_REQUIRE(a.tokens <= INT32_MAX - TPB && a.N <= INT32_MAX - CHUNK, PLA_B200_E_TOO_LARGE, "too many tokens or requests");
-  PLA_REQUIRE(a.query_start_loc && a.seq_lens && a.free_next && a.context_lens, PLA_B200_E_INVALID,
+  PLA_REQUIRE(a.query_start_loc && a.free_next && (a.N == 0 || (a.seq_lens && a.context_lens)), PLA_B200_E_INVALID,
               "context_lens, query_start_loc, seq_lens and free_next are required");
   PLA_REQUIRE(a.tokens == 0 || (a.slot_mapping && a.positions), PLA_B200_E_INVALID, "slot_mapping and positions are required");
   PLA_REQUIRE(a.N == 0 || a.columns == 0 || (a.block_table && a.table_row_stride >= a.columns), PLA_B200_E_INVALID,

@@ -118,13 +118,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_block_tables(
     const std::string bad = sanity_offsets(query_start_loc, num_tokens, 0);
     TORCH_CHECK(bad.empty(), "build_block_tables: sanity check: ", bad);
   }
-  if (N == 0) {                                  // no lengths to read: empty tensors have no address the entry could check
-    slots.fill_(-1);
-    positions.zero_();
-    if (free_start.has_value()) free_next.copy_(*free_start); else free_next.zero_();
-  } else if (!bypass_exec()) {
-    check_abi(pla_b200_block_tables(&g, stream_of(block_table)), "build_block_tables");
-  }
+  if (!bypass_exec()) check_abi(pla_b200_block_tables(&g, stream_of(block_table)), "build_block_tables");
   return {slots, positions, seq_lens, free_next};
 }
 

@@ -229,6 +229,21 @@ def test_tables_offsets_that_fall(native_built, context, new, first, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("requests", [0, 2])
+def test_tables_free_next_stays_inside_the_list(native_built, requests):
+    """Nothing to take: the next entry is the first one, at least 0 and at most the list's length, with and without requests."""
+    table, lens, offsets = torch.full((requests, 3), -7, dtype=torch.int32, device="cuda"), i32([4] * requests), i32([0] * (requests + 1))
+    for start, want in ((None, 0), (3, 3), (4, 4), (9, 4), (-5, 0)):
+        status = word()
+        plan = fa().build_block_tables(table, lens, offsets, i32([1, 2, 3, 5]), 4, num_tokens=300, free_start=None if start is None else i32([start]),
+                                       status=status)
+        assert plan.free_next.tolist() == [want] and status.item() == 0
+        assert plan.slot_mapping.tolist() == [-1] * 300 and plan.positions.tolist() == [0] * 300 and plan.seq_lens.tolist() == [4] * requests
+    plan = fa().build_block_tables(table, lens, offsets, i32([]), 4, num_tokens=0, free_start=i32([2]))
+    assert plan.free_next.tolist() == [0] and plan.slot_mapping.shape == (0,)
+
+
+@pytest.mark.gpu
 def test_tables_with_many_requests_and_streams(native_built):
     """More requests than one scan holds, several tiles of tokens; the same on another stream and replayed from a graph with other
     lengths in the same tensors."""
