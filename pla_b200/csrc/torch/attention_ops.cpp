@@ -8,6 +8,7 @@
 #include <tuple>
 
 #include "ops_common.h"
+#include "overlap.h"
 #include "pla_b200_attention.h"
 
 namespace pla_ops {
@@ -91,6 +92,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> build_block_tables(
   check_i32_vector(query_start_loc, N + 1, device, "query_start_loc");
   check_i32_vector(free_blocks, free_blocks.dim() == 1 ? free_blocks.size(0) : 0, device, "free_blocks");
   if (free_start.has_value()) check_i32_vector(*free_start, 1, device, "free_start");
+  Arguments args;
+  args.read(context_lens);
+  args.read(query_start_loc);
+  args.read(free_blocks);
+  args.read(free_start);
+  args.write(block_table, "block_table");
   TORCH_CHECK(block_size > 0 && block_size <= MAX_I32, "block_size must be positive");
   TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative");
   TORCH_CHECK(num_tokens < MAX_I32 / 2 && N < MAX_I32 / 2 && C < MAX_I32 && free_blocks.size(0) <= MAX_I32, "block tables: too many entries");
@@ -195,14 +202,30 @@ std::tuple<at::Tensor, at::Tensor> rotary(
   }
   c10::cuda::CUDAGuard guard(device);
   at::Tensor qo = out_rows(out_q, q, "out_q"), ko;
+  if (k.has_value() && !cached) ko = out_rows(out_k, *k, "out_k");
+  if (cached || out_q.has_value() || out_k.has_value()) {
+    Arguments args;
+    args.read(v);
+    args.read(q_weight);
+    args.read(k_weight);
+    args.read(positions);
+    args.read(inv_freq);
+    args.read(slot_mapping);
+    const int q_in = args.read(q), k_in = args.read(k);
+    if (out_q.has_value()) args.write(qo, "out_q", q_in);
+    if (out_k.has_value() && ko.defined()) args.write(ko, "out_k", k_in);
+    if (cached) {
+      args.write(*k_cache, "k_cache");
+      args.write(*v_cache, "v_cache");
+    }
+  }
   g.q = q.data_ptr();
   g.q_tok_stride = step(q, 0);
   g.q_head_stride = step(q, 1);
   g.q_out = qo.data_ptr();
   g.qo_tok_stride = step(qo, 0);
   g.qo_head_stride = step(qo, 1);
-  if (k.has_value() && !cached) {
-    ko = out_rows(out_k, *k, "out_k");
+  if (ko.defined()) {
     g.k_out = ko.data_ptr();
     g.ko_tok_stride = step(ko, 0);
     g.ko_head_stride = step(ko, 1);
@@ -274,6 +297,12 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_decode(const at::Tensor& q, c
   if (out.has_value()) {
     check_on(o, device, "out");
     TORCH_CHECK(o.is_contiguous() && o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type(), "out must be contiguous with q's shape and dtype");
+    Arguments args;
+    args.read(k_cache);
+    args.read(v_cache);
+    args.read(block_table);
+    args.read(seq_lens);
+    args.write(o, "out", args.read(q));
   }
   at::Tensor lse;
   if (return_lse) lse = fresh({B, Hq}, at::kFloat, device);

@@ -155,7 +155,7 @@ def apply_rotary(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotates the first ``2 * len(inv_freq)`` channels of every head of ``q`` ``[tokens, heads, dim]`` and ``k``
     by ``positions[t] * inv_freq`` and multiplies them by ``factor``; the other channels are copied. Pairs are ``(i, i + R/2)``, or
-    ``(2i, 2i + 1)`` with ``interleaved``. ``out_q=q`` / ``out_k=k`` rotate in place."""
+    ``(2i, 2i + 1)`` with ``interleaved``. ``out_q=q`` / ``out_k=k`` rotate in place; outputs that overlap anything else are refused."""
     if out_q is None and out_k is None:
         return _rotary(q, k, positions, inv_freq, factor, interleaved)
     return _rotary(q, k, positions, inv_freq, factor, interleaved, out_q, out_k)
@@ -204,7 +204,8 @@ def qk_norm_rotary_cache(
 ) -> torch.Tensor:
     """:func:`qk_norm_rotary` whose keys go to ``k_cache[slot // block_size, slot % block_size]`` (``[blocks, block_size, kv heads, dim]``
     with any strides) and whose values are copied to ``v_cache`` likewise; returns the queries. A negative slot stores
-    nothing; a slot outside the pool stores nothing and sets 8 in ``status``. The slots of a call must differ."""
+    nothing; a slot outside the pool stores nothing and sets 8 in ``status``. The slots of a call must differ, and the caches must not
+    overlap each other or the rows."""
     if out_q is None and status is None:
         return _norm_rotary_cache(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, slot_mapping, eps, factor, interleaved,
                                   unit_offset)
@@ -230,7 +231,7 @@ def paged_attention_decode(
     natural log of the softmax sums in fp32.
 
     ``status`` (int32[1]) gets 1 for a length that is negative or past the table's row, 8 for a page outside the pool (its
-    tokens are left out)."""
+    tokens are left out). ``out`` is contiguous; it may be ``q``."""
     if out is None and status is None:
         o, lse = _paged_decode(q, k_cache, v_cache, block_table, seq_lens, scale, return_lse)
     else:

@@ -782,6 +782,68 @@ def test_attention_refusals(native_built):
 
 
 @pytest.mark.gpu
+def test_overlapping_outputs_are_refused(native_built):
+    """What a call writes may be its own input, element for element, and nothing else that the call reads or writes; no row of it twice."""
+    T, D, bf = 6, 64, dict(dtype=torch.bfloat16, device="cuda")
+    freq, pos, w = torch.ones(8, dtype=torch.float64, device="cuda"), torch.arange(T, device="cuda"), torch.ones(D, device="cuda")
+    flat = torch.randn(4 * T * 4 * D, **bf)
+    q, k = torch.randn(T, 4, D, **bf), torch.randn(T, 4, D, **bf)
+    row = flat[:T * 12 * D].view(T, 12, D)
+    for kw in [dict(out_q=q[:1].expand(T, 4, D)), dict(out_q=q[:, :1].expand(T, 4, D)), dict(out_k=k[:1].expand(T, 4, D)), dict(out_q=k), dict(out_k=q),
+               dict(out_q=q, out_k=q), dict(out_q=row[:, :4], out_k=row[:, 2:6]), dict(out_q=row[:, 8:], out_k=row[:, 8:]), dict(out_q=k, out_k=row[:, :4]), dict(out_q=row[:, :4], out_k=q),
+               dict(out_q=flat.as_strided((T, 4, D), (3 * D, D, 1)))]:
+        for call in (lambda: fa().apply_rotary(q, k, pos, freq, **kw), lambda: fa().qk_norm_rotary(q, k, w, w, pos, freq, **kw)):
+            with pytest.raises(RuntimeError, match="overlap"):
+                call()
+    with pytest.raises(RuntimeError, match="overlap"):                           # a row further on in the same tensor
+        fa().apply_rotary(flat[:T * 4 * D].view(T, 4, D), None, pos, freq, out_q=flat[4 * D:(T + 1) * 4 * D].view(T, 4, D))
+    with pytest.raises(RuntimeError, match="overlap"):
+        fa().apply_rotary(q[:1].expand(T, 4, D), None, pos, freq, out_q=q[:1].expand(T, 4, D))
+    cache = torch.randn(3, 2, 16, 4, D, **bf)
+    kc, vc = cache[:, 0], cache[:, 1]
+    slots = torch.arange(T, device="cuda")
+    rest = dict(q=q, k=k, v=k, q_weight=w, k_weight=w, positions=pos, inv_freq=freq, k_cache=kc, v_cache=vc, slot_mapping=slots)
+    for over in [dict(v_cache=kc), dict(k_cache=kc[:1].expand(3, 16, 4, D)), dict(v_cache=vc[:, :1].expand(3, 16, 4, D)), dict(k=kc[0, :T]), dict(v=kc[0, :T]),
+                 dict(q=vc[1, :T]), dict(out_q=vc[1, :T]), dict(out_q=k), dict(v_cache=cache.flatten(0, 1)[1:4])]:
+        with pytest.raises(RuntimeError, match="overlap"):
+            fa().qk_norm_rotary_cache(**(rest | over))
+    table, lens = i32([[0, 1]] * T), i32([5] * T)
+    for out in (kc[0, :T], flat[:T * 4 * D].view(T, 4, D)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            fa().paged_attention_decode(flat[D:D + T * 4 * D].view(T, 4, D) if out.data_ptr() == flat.data_ptr() else q, kc, vc, table, lens, out=out)
+    both = torch.arange(12, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        fa().build_block_tables(both[:4].view(2, 2), i32([0, 0]), i32([0, 1, 2]), both[3:], 4, num_tokens=2)
+
+
+@pytest.mark.gpu
+def test_in_place_and_interleaved_views(native_built):
+    """Outputs that are their inputs, or lie between them: parts of one packed row, heads side by side, heads outermost, halves of one
+    cache, the attention's output in place of its queries. The same bits as with tensors of their own."""
+    T, H, D, bf = 70, 4, 128, dict(dtype=torch.bfloat16, device="cuda")
+    freq, pos, w = fa().rotary_frequencies(64)[0].cuda(), torch.arange(T, device="cuda"), torch.rand(D, device="cuda")
+    fresh = torch.randn(3, T, H, D, **bf)
+    want = fa().qk_norm_rotary(fresh[0], fresh[1], w, w, pos, freq)
+    packed = torch.cat([x.flatten(1) for x in fresh], 1).contiguous()
+    side = torch.stack(list(fresh), 2)                                            # [T, H, 3, D]
+    outer = fresh.transpose(1, 2).contiguous()                                    # [3, H, T, D]
+    for q, k, v in ((packed[:, :H * D].unflatten(1, (H, D)), packed[:, H * D:2 * H * D].unflatten(1, (H, D)), packed[:, 2 * H * D:].unflatten(1, (H, D))),
+                    (side[:, :, 0], side[:, :, 1], side[:, :, 2]), [x.transpose(0, 1) for x in outer]):
+        cache = torch.zeros(6, 2, 16, H, D, **bf)
+        out = fa().qk_norm_rotary_cache(q, k, v, w, w, pos, freq, cache[:, 0], cache[:, 1], torch.arange(T, device="cuda"), out_q=q)
+        assert out.data_ptr() == q.data_ptr() and torch.equal(q, want[0])
+        assert torch.equal(cache[:, 0].flatten(0, 1)[:T], want[1]) and torch.equal(cache[:, 1].flatten(0, 1)[:T], fresh[2])
+        fa().qk_norm_rotary(v, k, w, w, pos, freq, out_q=v, out_k=k)
+        assert torch.equal(k, want[1]) and torch.equal(v, fa().qk_norm_rotary(fresh[2], None, w, None, pos, freq)[0])
+    for lens, hq, hk, columns in ([70, 0, 500, 33], 16, 2, 2), ([70, 0, 2000, 33], 16, 2, 1000), ([900] * 40, 8, 8, 0):
+        q, kc, vc, table = paged_inputs(9, lens, hq, hk, 128, 16, extra_columns=columns)
+        want = fa().paged_attention_decode(q.cuda(), kc, vc, table.cuda(), i32(lens))
+        x = q.cuda()
+        got = fa().paged_attention_decode(x, kc, vc, table.cuda(), i32(lens), out=x)
+        assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_sanity_check_names_bad_metadata(native_built, monkeypatch):
     monkeypatch.setenv("PLA_SANITY_CHECK", "1")
     q, kc = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
