@@ -120,6 +120,33 @@ __device__ __forceinline__ float rsqrt_fast(float x) {     // relative error wit
   return y;
 }
 
+// 1 / sqrt(mean(x^2) + eps) of a row whose squares leave the range of 32-bit numbers (bf16 rows of magnitude 1e-20 with a tiny eps, or of
+// 1e20), as two factors: a power of two that brings the row's largest number, or the root of eps, to about 1, and the rest. The lane's
+// pieces of the row are read again, so that ordinary rows keep nothing for it.
+template <typename act_t, int GROUP>
+__device__ __forceinline__ float2 inverse_scaled(const uint4* low, const uint4* high, float inv_d, float eps) {
+  const float root = sqrtf(eps);
+  float most = root, sq = 0.0f, x[8];
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    unpack<act_t>(c == 0 ? *low : *high, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+  }
+#pragma unroll
+  for (int o = GROUP / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float scale = __int_as_float(max(254 - (__float_as_int(most) >> 23), 1) << 23);       // 2^(127 - exponent); infinity: 2^-126
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    unpack<act_t>(c == 0 ? *low : *high, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sq = fmaf(x[i] * scale, x[i] * scale, sq);
+  }
+#pragma unroll
+  for (int o = GROUP / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  return make_float2(scale, rsqrt_fast(fmaf(sq, inv_d, root * scale * (root * scale))));
+}
+
 template <typename act_t, int GROUP, int LAYOUT>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) rotary_kernel(const __grid_constant__ Work p) {
   constexpr int ROWS = 32 / GROUP;                     // rows per step of a warp
@@ -423,7 +450,14 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) rotary_kernel(const __grid
           for (int i = 0; i < 16; ++i) sq = fmaf(x[i / 8][i % 8], x[i / 8][i % 8], sq);
 #pragma unroll
           for (int o = GROUP / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float inv = rsqrt_fast(fmaf(sq, inv_d, p.eps));
+          const float mean = fmaf(sq, inv_d, p.eps);
+          float inv = rsqrt_fast(mean);
+          if (__any_sync(0xffffffffu, !(mean >= 0x1p-100f && mean < INFINITY))) {
+            const float2 two = inverse_scaled<act_t, GROUP>(&s_ring[warp][cell][0][lane], &s_ring[warp][cell][1][lane], inv_d, p.eps);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i / 8][i % 8] *= two.x;
+            inv = two.y;
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i / 8][i % 8] *= inv;
         }

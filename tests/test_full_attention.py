@@ -366,6 +366,31 @@ def test_norm_rotary_matches_the_oracle(native_built, T, hq, hk, D, R, inter, un
     assert torch.equal(dq, oq) and torch.equal(dk, ok)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("D,R,inter", [(128, 64, False), (128, 128, False), (256, 128, True), (96, 72, False), (64, 20, True)])
+def test_norm_of_very_small_and_large_rows(native_built, D, R, inter, eps):
+    """bf16 rows whose squares are no 32-bit numbers, next to ordinary rows: the norm of the definition, in the bounds of every other row. The
+    mean of the squares is taken of rows that are scaled by a power of two, so nothing is added to the bound."""
+    sizes = [1.0, 1e-15, 1e-19, 1e-23, 1e-30, 1e-37, 1e19, 1e23, 1e30, 1e36, 3.0]
+    g = torch.Generator().manual_seed(D)
+    x = (torch.randn(5, len(sizes), D, generator=g) * torch.tensor(sizes)[:, None]).bfloat16()
+    if eps > 0:
+        x[:, 0] = 0
+    w, pos = torch.rand(D, generator=g) + 0.5, torch.arange(5) * 100
+    freq = 10000.0 ** (-torch.arange(R // 2, dtype=torch.float64) * 2 / R)
+    got, _ = fa().qk_norm_rotary(x.cuda(), None, w.cuda(), None, pos.cuda(), freq.cuda(), eps=eps, interleaved=inter)
+    y, bound = expect(x, w, pos, freq, inter, eps=eps)
+    assert_within(got, y, bound + 2.0 ** -134)            # and half the smallest step of bf16
+    x[1, 3, 5], x[2, 7, 9], x[3, 0, 0] = float("inf"), float("nan"), float("-inf")
+    got, _ = fa().qk_norm_rotary(x.cuda(), None, w.cuda(), None, pos.cuda(), freq.cuda(), eps=eps, interleaved=inter)
+    spoilt = torch.zeros(x.shape[:2], dtype=torch.bool)
+    spoilt[1, 3] = spoilt[2, 7] = spoilt[3, 0] = True
+    assert torch.equal((~torch.isfinite(got)).any(-1).cpu(), spoilt)
+    assert got[2, 7].isnan().all()
+    assert_within(got.cpu()[~spoilt], y[~spoilt], bound[~spoilt] + 2.0 ** -134)
+
+
 def caches(blocks, bs, hk, D, dtype, layout, fill=float("nan")):
     """k and v caches of one of three layouts, addressed [page, token, head, channel]."""
     if layout == "packed":
