@@ -137,6 +137,8 @@ def rotary_frequencies(
         low = max(math.floor(channel(beta_fast)), 0)
         high = min(math.ceil(channel(beta_slow)), rotary_dim - 1)
         keep = 1.0 - ((index - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        if channel(beta_slow) < 0.0:                 # even the first channel turns fewer than beta_slow times
+            keep = torch.zeros_like(index)
         freq = freq * keep + freq / factor * (1.0 - keep)
         multiply = 0.1 * math.log(factor) + 1.0
     return freq.to(device), multiply

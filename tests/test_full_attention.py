@@ -72,6 +72,15 @@ def test_frequencies_plain_and_scaled(native_built):
     assert (yarn[1:] < yarn[:-1]).all()
 
 
+@pytest.mark.parametrize("original,fast,slow", [(4, 32.0, 1.0), (128, 64.0, 32.0), (1, 2.0, 0.5)])
+def test_yarn_divides_every_slow_channel(native_built, original, fast, slow):
+    """A context so short that even the fastest channel turns fewer than beta_slow times: all of them are divided, the first one too."""
+    plain, _ = fa().rotary_frequencies(64, 10000.0)
+    assert original / (2 * math.pi) < slow
+    yarn, _ = fa().rotary_frequencies(64, 10000.0, scaling="yarn", factor=8.0, original_max_position=original, beta_fast=fast, beta_slow=slow)
+    torch.testing.assert_close(yarn, plain / 8, rtol=1e-15, atol=0)
+
+
 @pytest.mark.parametrize("kw", [dict(rotary_dim=0), dict(rotary_dim=7), dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, scaling="other"),
                                 dict(rotary_dim=8, factor=0.5), dict(rotary_dim=2, scaling="ntk", factor=2.0),
                                 dict(rotary_dim=8, scaling="yarn", beta_fast=1.0, beta_slow=2.0),
