@@ -22,6 +22,9 @@ at::Tensor fresh(at::IntArrayRef size, at::ScalarType dtype, const at::Device& d
   return at::detail::empty_cuda(size, dtype, device, std::nullopt);
 }
 
+// The kernels take scalars as 32-bit numbers.
+bool finite32(double x) { return std::isfinite(static_cast<float>(x)); }
+
 void check_on(const at::Tensor& t, const at::Device& device, const char* name) {
   TORCH_CHECK(t.device() == device, name, " must be on ", device, ", got ", t.device());
 }
@@ -171,7 +174,8 @@ std::tuple<at::Tensor, at::Tensor> rotary(
   TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.is_contiguous(),
               "inv_freq must be a contiguous 1-D float64 tensor (rotary_frequencies makes it)");
   TORCH_CHECK(2 * inv_freq.size(0) <= D, "the rotated part (2 * inv_freq entries) must be at most the head size");
-  TORCH_CHECK(std::isfinite(eps) && eps >= 0.0 && std::isfinite(factor), "eps must be finite and non-negative, factor finite");
+  TORCH_CHECK(finite32(eps) && eps >= 0.0 && (eps == 0.0 || static_cast<float>(eps) > 0.0f) && finite32(factor),
+              "eps must be finite and non-negative, factor finite, both as 32-bit numbers");
   g.positions = index_view(positions, T, device, "positions");
   g.inv_freq = inv_freq.data_ptr<double>();
   g.q_weight = norm_weight(q_weight, D, device, "q_weight", &g.q_weight_dtype);
@@ -291,7 +295,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_decode(const at::Tensor& q, c
   TORCH_CHECK(block_table.size(1) <= 1 || block_table.stride(1) == 1, "block_table columns must be contiguous");
   TORCH_CHECK(block_table.size(1) <= MAX_I32, "block_table has too many columns");
   check_i32_vector(seq_lens, B, device, "seq_lens");
-  TORCH_CHECK(!scale.has_value() || std::isfinite(*scale), "scale must be finite");
+  TORCH_CHECK(!scale.has_value() || finite32(*scale), "scale must be finite as a 32-bit number");
   c10::cuda::CUDAGuard guard(device);
   at::Tensor o = out.has_value() ? *out : fresh({B, Hq, D}, q.scalar_type(), device);
   if (out.has_value()) {

@@ -816,6 +816,18 @@ def test_attention_refusals(native_built):
 
 
 @pytest.mark.gpu
+def test_scalars_outside_32_bits_are_refused(native_built):
+    q, kc = torch.ones(1, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(2, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    freq, w = torch.ones(4, dtype=torch.float64, device="cuda"), torch.ones(64, device="cuda")
+    for scale in (1e39, -1e300, math.nan):
+        with pytest.raises(RuntimeError, match="scale"):
+            fa().paged_attention_decode(q, kc, kc, i32([[0]]), i32([3]), scale=scale)
+    for kw in (dict(factor=1e39), dict(factor=math.nan), dict(eps=1e39), dict(eps=1e-60), dict(eps=-1e-6), dict(eps=math.nan)):
+        with pytest.raises(RuntimeError, match="32-bit"):
+            fa().qk_norm_rotary(q, None, w, None, i32([0]), freq, **kw)
+
+
+@pytest.mark.gpu
 def test_overlapping_outputs_are_refused(native_built):
     """What a call writes may be its own input, element for element, and nothing else that the call reads or writes; no row of it twice."""
     T, D, bf = 6, 64, dict(dtype=torch.bfloat16, device="cuda")
