@@ -828,6 +828,28 @@ def test_scalars_outside_32_bits_are_refused(native_built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("hq,hk,D,R", [(1, 1, 8, 2), (32, 8, 128, 128), (16, 2, 256, 64), (5, 1, 96, 48), (3, 2, 128, 40), (2, 1, 64, 20)])
+def test_one_token_is_rotated(native_built, hq, hk, D, R, inter, dtype):
+    """A decode step's rotation, at positions where no angle is a whole turn; with the norm and without."""
+    g = torch.Generator().manual_seed(D + R)
+    row, (q, k, _) = rows(g, 1, hq, hk, D, DT[dtype])
+    w = torch.rand(D, generator=g) + 0.5
+    freq = 10000.0 ** (-torch.arange(R // 2, dtype=torch.float64) * 2 / R)
+    dq, dk, _ = on_gpu(row, hq, hk, D)
+    for position in (1, 777777, -5):
+        pos = torch.tensor([position])
+        for weight in (None, w):
+            dw = None if weight is None else weight.cuda()
+            got = fa().qk_norm_rotary(dq, dk, dw, dw, pos.cuda(), freq.cuda(), interleaved=inter)
+            for x, y, name in zip((q, k), got, "qk"):
+                want, bound = expect(x, weight, pos, freq, inter)
+                assert_within(y, want, bound, name)
+                assert weight is not None or not torch.equal(y.cpu(), x)
+
+
+@pytest.mark.gpu
 def test_overlapping_outputs_are_refused(native_built):
     """What a call writes may be its own input, element for element, and nothing else that the call reads or writes; no row of it twice."""
     T, D, bf = 6, 64, dict(dtype=torch.bfloat16, device="cuda")
