@@ -17,17 +17,22 @@ struct Runs {
 
   Runs() = default;
   explicit Runs(const at::Tensor& t) {
-    const int64_t bytes = t.element_size();
-    at = static_cast<int64_t>(reinterpret_cast<intptr_t>(t.data_ptr()));
+    const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+    const int64_t bytes = static_cast<int64_t>(t.element_size());
+    at = static_cast<int64_t>(reinterpret_cast<intptr_t>(t.const_data_ptr()));
     empty = t.numel() == 0;
     run = bytes;
-    for (int64_t d = 0; d < t.dim(); ++d) add(t.size(d), t.stride(d) * bytes);
+    for (size_t d = sizes.size(); d-- > 0;) add(sizes[d], strides[d] * bytes);
     fold();
   }
-  // One more axis, kept in order of stride; views have few.
+  // One more axis, kept in order of stride; views have few, and come innermost axis first.
   void add(int64_t n, int64_t step) {
     if (n <= 1) return;
-    TORCH_CHECK(axes < MOST, "views of more than ", MOST, " axes are not supported");
+    if (axes == MOST) TORCH_CHECK(false, "views of more than ", MOST, " axes are not supported");
+    if (axes == 0 && step == run) {        // the usual innermost axis
+      run *= n;
+      return;
+    }
     int i = axes++;
     for (; i > 0 && stride[i - 1] < step; --i) size[i] = size[i - 1], stride[i] = stride[i - 1];
     size[i] = n, stride[i] = step;
@@ -71,11 +76,7 @@ inline bool apart(const Runs& a, const Runs& b) { return a.empty || b.empty || a
 class Arguments {
  public:
   // Each returns the argument's number, -1 for one that is not given.
-  int read(const at::Tensor& t) {
-    TORCH_CHECK(count_ < MOST, "too many arguments");
-    seen_[count_] = Runs(t);
-    return count_++;
-  }
+  int read(const at::Tensor& t) { return add(Runs(t)); }
   int read(const std::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? read(*t) : -1; }
   // A tensor of the caller's that is written: its elements must not overlap each other, nor anything added so far. It may be argument
   // `in_place`, element for element, where every row is read before it is written.
@@ -85,10 +86,15 @@ class Arguments {
     for (int i = 0; i < count_; ++i)
       TORCH_CHECK(apart(mine, seen_[i]) || (i == in_place && mine.same(seen_[i])), name, " overlaps another argument",
                   in_place >= 0 ? " (it may be its own input, element for element)" : "");
-    return read(t);
+    return add(mine);
   }
 
  private:
+  int add(const Runs& r) {
+    TORCH_CHECK(count_ < MOST, "too many arguments");
+    seen_[count_] = r;
+    return count_++;
+  }
   static constexpr int MOST = 12;
   Runs seen_[MOST];
   int count_ = 0;
