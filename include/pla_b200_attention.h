@@ -94,8 +94,10 @@ int pla_b200_rotary(const pla_b200_rotary_args* args, void* stream);
  * Attention of one new token per request over a paged key/value cache:
  *   s_j = scale * q . k_j,  j < seq_lens[b];  lse = log(sum exp(s_j));  out = sum exp(s_j - lse) v_j
  * Query head h reads key/value head h / (Hq / Hk). A request of length 0 gets zeros and lse = -inf. Token j sits in page
- * block_table[b, j / block_size]; nothing at or past seq_lens[b] is read. A length < 0 (taken as 0) or past the table's
- * columns or 2^30 (cut there) sets PLA_B200_DEV_BAD_INTERVAL; tokens whose page lies outside the pool are left out and set PLA_B200_DEV_BAD_SLOT.
+ * block_table[b, j / block_size]. Tokens at or past seq_lens[b] never reach the result, but up to 15 rows behind it in the last
+ * page may be read; table entries past the request's pages are not. A length < 0 (taken as 0) or past the table's columns or 2^30
+ * (cut there) sets PLA_B200_DEV_BAD_INTERVAL; tokens whose page lies outside the pool are left out and set PLA_B200_DEV_BAD_SLOT.
+ * NaN scores make the outputs and lse that they are part of NaN. `out` may be q itself when q is dense.
  * ======================================================================== */
 typedef struct pla_b200_paged_decode_args {
   const void* q;        /* [B, Hq, D] */

@@ -6,7 +6,7 @@
 // (p % block_size == 0) is the one that writes the page's table entry: a page taken by this call always starts with a
 // token of this call, because the context's last page is held already.
 // The call moves a few bytes per request and 16 per token: what bounds it is the chain of dependent reads (lengths ->
-// scan -> free list -> stores) behind one launch.
+// scan -> free list -> stores) behind one launch (256 requests with one token each 3.3 us, 8 with 40K tokens the same).
 #include "common.cuh"
 #include "../../include/pla_b200_attention.h"
 

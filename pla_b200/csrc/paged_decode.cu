@@ -15,12 +15,14 @@
 // tensor map over the cache, one copy per 64 channels; other page sizes take two producer warps and 16-byte asynchronous copies from
 // each row's page (32 requests up to 8K tokens of 8 heads of 128: 93 us in pages of one token, 85 is the floor). Both
 // leave the 128-byte swizzle that ldmatrix reads without bank conflicts. Tried before: one bulk copy per row and lane (the lanes' copies
-// issue one after another, 480 of 620 instructions per tile of 16 tokens) and every warp loading for itself (290 per tile, here 240).
+// issue one after another, 480 of 620 instructions per tile of 16 tokens) and every warp loading for itself (290 per tile against 240).
 // A part that begins or ends inside a CTA's range goes to the workspace as 32-bit sums, and a second kernel, launched so that it
 // waits on the first one's end only, joins the parts in order: no atomics, the same bits every time. Calls with little work go to
 // clusters instead, which join their parts through distributed shared memory in the same kernel.
-// Device time on a B200: 64 requests up to 16K tokens, 16/2 heads of 256 (1.14 GB) 177 us, 6.4 TB/s; one of 128K, 32/8 heads of 128 (0.54 GB)
-// 91 us, 5.9 TB/s; 250 up to 2K, 32/4 heads of 64 (0.28 GB) 58 us, 4.9 TB/s; 8 up to 4K, 32/8 of 128 (71 MB) 21 us; one of 777, 16/2 of 128 5.4 us.
+// Device time on a B200, calls captured one after another: 64 requests up to 16K tokens, 16/2 heads of 256 (1.14 GB) 177 us, 6.4 TB/s (192 us
+// after half a second of such calls, when the 1,000 W cap has the SMs at 1,815 MHz); one of 128K, 32/8 heads of 128 (0.54 GB) 91 us, 5.9 TB/s; 250 up to 2K,
+// 32/4 heads of 64 (0.28 GB) 59 us, 4.8 TB/s; 8 up to 4K, 32/8 of 128 (71 MB) 21 us; one of 777, 16/2 of 128 5.6 us. More than 16 query heads per
+// key/value head read the rows once per 16: 16 requests up to 16K, heads of 128, 24 us with 16/1 heads, 48 with 64/1, 11 is the floor of both.
 // What is left: about 5 us until a CTA's first rows arrive (lengths, page table and rows are three reads that depend on each other), 10 %
 // between the first and the last CTA to finish (SMs get unequal shares of the bandwidth), and 4 us for the join. Handing out the last
 // eighth or quarter of the units from a counter evened the CTAs out, but the additional parts cost the join more (91 -> 109 us for 128K);
@@ -29,7 +31,9 @@
 // what the rounding left, and V is multiplied by both: relative 2^-16 (bf16) or 2^-22 (fp16), far below the output's own rounding.
 // fp16 loses small numbers, so its weights are 2^7 (SHIFT) times as large: what is lost of one is at most 2^-32 of the largest. The matrix unit
 // cuts every product at about 2^-24 of the number that it adds to, which loses a long tail of small weights behind a large one: the 16
-// tokens of a tile are summed from zero, and that sum is added in 32 bits, rounded to nearest.
+// tokens of a tile are summed from zero, and that sum is added in 32 bits, rounded to nearest. Both together cost the first case 28 %
+// more instructions and no time, 3 to 4 % under the power cap, and 9 % in the 64/1 case, whose rows come from L2; packed additions
+// (add.f32x2), tiles in groups of two or four and accumulators that begin as constants changed nothing or lost.
 #include <cuda.h>
 
 #include <type_traits>
@@ -215,6 +219,8 @@ __device__ __forceinline__ float4 team_load4(uint32_t addr) {
   return x;
 }
 
+// Sixteen query heads at once (NT = 2) with 96, 128 or 256 channels take every register there is, and ptxas spills up to 56 bytes (16 requests
+// up to 16K, 32/2 heads of 256: 62 us, 4.7 TB/s).
 // Warps that load: rows one by one take two (64 requests up to 8K tokens of 4 heads of 64 67 -> 59 us, of 2 heads of 256 137 -> 98), except
 // where the computing warps need the registers (16 query heads of 64, three CTAs per SM: 41.8 us with one, 43.9 with two).
 template <int D, int NT, bool BOXED>

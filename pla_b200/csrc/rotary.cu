@@ -11,8 +11,8 @@
 // (in 32 bits whole radians are lost at positions of a million), take sine and cosine in 32 bits and share them through shared
 // memory. Warps are persistent and bring the next rows, of the next token as well, through a ring of 16-byte asynchronous copies,
 // each lane into cells of its own.
-// On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 112 us, 6.0 TB/s; rotation alone of 32,761
-// tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 119 us, 5.6 TB/s; 1,999 tokens with the norm (41 MB) 12 us; one token 3 us. At 2.6
+// On a B200: norm, rotation (64 of 256) and cache write of 32K tokens of 16/2 heads (671 MB) 115 to 120 us, 5.6 to 5.8 TB/s; rotation alone of
+// 32,761 tokens, 64 of 128 interleaved, 32/8 heads (671 MB) 118 us, 5.7 TB/s; 1,999 tokens with the norm (41 MB) 12 us; one token 3 us. At 2.6
 // instructions per cycle and SM the arithmetic alone takes about 75 us of these; a seventh fewer instructions did not shorten the large
 // calls, so what is left is how well reads and writes overlap. Measured and not kept: two channels per instruction (fma.f32x2: the
 // register pairs cost more moves than it saves, 61 -> 83 million instructions for the interleaved case), three CTAs per SM (80 registers

@@ -8,7 +8,7 @@ adding eight and five shuffle steps, 13 * 2^-24, its root and two products: 2^-2
 scores are 32-bit sums of D products, off by at most D * 2^-24 * scale * sum |q| |k| =: e; the weights are rounded to the activations'
 type for the product with v, and the 32-bit sums over n tokens are off by at most (n + 64) * 2^-24, so an output is
 within (half + 2 e + 2 (n + 64) 2^-24 + 2^-20) * sum p |v|, plus its own rounding; the log of the sum within e + (n + 64) 2^-24 +
-2^-22 (1 + |lse|)."""
+2^-22 (1 + |lse|). The kernel holds the weights in two numbers of the activations' type; ``assert_attention_kept`` bounds that."""
 import math
 
 import pytest
