@@ -32,8 +32,8 @@ typedef struct pla_b200_page_strides {
  * block_table[n, p / block_size] * block_size + p % block_size. Other entries of the table keep their values. Tokens at or past
  * query_start_loc[N], tokens without a page and tokens of a request with bad metadata (c < 0, m < 0, c + m past 32 bits, or an
  * offset query_start_loc[n] that is negative or below an earlier one: it takes no pages, seq_lens[n] = max(c, 0),
- * PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last kind. A page past the end of the free list becomes -1. `tokens` has to cover query_start_loc[N], which has to be the largest offset; new tokens past
- * either are left out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs
+ * PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last kind. A page past the end of the free
+ * list becomes -1. `tokens` has to cover query_start_loc[N], which has to be the largest offset; new tokens past either are left out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs
  * (block_table is both).
  * ======================================================================== */
 typedef struct pla_b200_block_tables_args {
@@ -42,11 +42,11 @@ typedef struct pla_b200_block_tables_args {
   const int32_t* context_lens;    /* [N] tokens already in the cache */
   const int32_t* query_start_loc; /* [N + 1] offsets of the new tokens */
   const int32_t* free_blocks;     /* [free_count] */
-  const int32_t* free_start;      /* [1] first entry of the list that is still free, or NULL (0) */
+  const int32_t* free_start;      /* [1] first entry of the list that is still free (below 0: 0), or NULL (0) */
   int64_t* slot_mapping;          /* [tokens] */
   int64_t* positions;             /* [tokens] */
   int32_t* seq_lens;              /* [N]: c + m */
-  int32_t* free_next;             /* [1]: first entry that is free after this call */
+  int32_t* free_next;             /* [1]: first entry that is free after this call, at most free_count */
   int32_t N, tokens, columns, free_count, block_size;
   int32_t* status;
 } pla_b200_block_tables_args;
@@ -60,7 +60,8 @@ int pla_b200_block_tables(const pla_b200_block_tables_args* args, void* stream);
  * with (a, b) = (i, i + R/2), or (2i, 2i + 1) when interleaved. Angles are reduced to one turn in 64 bits; one rounding at the end.
  * k may be absent (Hk = 0). With k_cache (then k_out is NULL), k rows go to their slots and v rows
  * are copied to theirs; a slot < 0 stores nothing, a slot outside the pool sets PLA_B200_DEV_BAD_SLOT. Slots of one call
- * must differ. q_out / k_out may be q / k themselves. Rows and strides are multiples of 16 bytes.
+ * must differ. q_out / k_out may be q / k themselves; otherwise nothing that is written may overlap anything else. Rows and
+ * strides are multiples of 16 bytes.
  * ======================================================================== */
 typedef struct pla_b200_rotary_args {
   const void* q;       /* [T, Hq, D] */

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(TPB) block_tables_kernel(const pla_b200_block_
         s_ctx[tid * PER + i] = -1;
       } else {
         // tokens without a row have no thread that could enter a page for them: they are left out of everything
-        const int len = ctx[i] + min(off[i + 1], rows) - min(off[i], rows), all = pages(len);
+        const int len = ctx[i] + (min(off[i + 1], rows) - min(off[i], rows)), all = pages(len);
         need[i] = max(min(all, p.columns) - pages(ctx[i]), 0);
         if (off[i + 1] > rows) bad |= PLA_B200_DEV_BAD_INTERVAL;
         if (all > p.columns) bad |= PLA_B200_DEV_TABLE_FULL;

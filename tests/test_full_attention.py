@@ -220,6 +220,8 @@ def test_tables_leave_out_tokens_without_a_row(native_built):
     assert want[5] == 1 and want[3][667:] == [i % 9 for i in range(667, 1500)]
     want = tables_case([5, 2 ** 31 - 3], [1, 3], 1 << 20, columns=4)              # a length past 32 bits
     assert want[5] == 1 and want[3] == [6, 2 ** 31 - 3] and want[1][1:] == [-1] * 3
+    want = tables_case([0, 2 ** 31 - 10], [900, 9], 1 << 20, columns=4)           # one that just fits, behind other tokens
+    assert want[5] == 64 and want[3] == [900, 2 ** 31 - 1] and want[1][900:] == [-1] * 9
 
 
 @pytest.mark.gpu
