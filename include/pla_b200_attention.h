@@ -33,7 +33,8 @@ typedef struct pla_b200_page_strides {
  * query_start_loc[N], tokens without a page and tokens of a request with bad metadata (c < 0, m < 0, c + m past 32 bits, or an
  * offset query_start_loc[n] that is negative or below an earlier one: it takes no pages, seq_lens[n] = max(c, 0),
  * PLA_B200_DEV_BAD_INTERVAL) get slot -1; position 0 for the first and the last kind. A page past the end of the free
- * list becomes -1. `tokens` has to cover query_start_loc[N], which has to be the largest offset; new tokens past either are left out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs
+ * list becomes -1. `tokens` has to cover query_start_loc[N], which has to be the largest offset; new tokens past either are left
+ * out of m, pages, table, seq_lens and free_next alike (PLA_B200_DEV_BAD_INTERVAL). Outputs must not overlap inputs
  * (block_table is both).
  * ======================================================================== */
 typedef struct pla_b200_block_tables_args {
